@@ -231,6 +231,52 @@ GQ_API int gq_embedding_rows(int32_t type, const void* src, size_t src_bytes, in
 GQ_API int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* codes, uint16_t* scales_bf16,
                             void* stream);
 
+/* Block-scaled 8-bit floats: e4m3 codes and power-of-two scales stored as E8M0 bytes
+ * (byte b = 2^(b - 127)).  A block's scale is 2^e with the smallest e >= -127 for which its
+ * largest finite magnitude is at most 448 * 2^e (e = 0 when that is 0); a code is the value
+ * over the scale rounded to nearest even, and a value that is not finite becomes the NaN
+ * code and leaves the rest of its block as it is.  No counterpart in the reference, whose
+ * weights stay integer (gguf_conversion.py:102-176) and whose products run on the Modalix
+ * accelerator (ModelGraph.linear, sima_lmm/model/model_graph.py:351-403): these four run a
+ * GGUF file's projections on the GPU itself.  Device pointers of the current device; all
+ * strides are in elements, and the elements of a row are consecutive.  Shapes with a zero
+ * extent do nothing, except that a product over k = 0 is the bias (or 0).
+ *
+ * gq_convert_fp8: a GGUF tensor (any type of gq_convert, perm_heads included; cols a
+ * multiple of 32) to tensor->codes, rows * cols e4m3 bytes, and scales, one per 128 x 128
+ * block: (ceil(rows/128), ceil(cols/128)), row-major.  The values quantized are the f32
+ * ones of GQ_OUT_F32.  tensor->scales, values and diag are not used.  src and codes 16-byte
+ * aligned. */
+GQ_API int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream);
+
+/* RMS norm of rows, quantized: h = x + residual rounded to the input type (h = x when
+ * residual is NULL), y = h / sqrt(mean(h^2) + eps) * weight in f32, y as e4m3 codes
+ * (rows, cols) with one scale per 1 x 128 block (rows, ceil(cols/128)).  dtype (of x,
+ * residual and sum): GQ_TYPE_F32, F16 or BF16; weight: f32 (cols).  sum receives h when
+ * residual is given and may be residual or x itself.  cols a multiple of 32; rows at most
+ * 2^31 - 1; every row of x, residual, sum and codes starts on a 16-byte boundary, and weight
+ * does. */
+GQ_API int gq_rms_norm_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_residual,
+                           const float* weight, float eps, int64_t rows, int64_t cols, void* sum, int64_t ld_sum,
+                           uint8_t* codes, int64_t ld_codes, uint8_t* scales, int64_t ld_scales, void* stream);
+
+/* Rows quantized the same way: x, or silu(gate) * x = gate / (1 + exp(-gate)) * x in f32 when
+ * gate is given.  Same types and alignment. */
+GQ_API int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* gate, int64_t ld_gate,
+                           int64_t rows, int64_t cols, uint8_t* codes, int64_t ld_codes, uint8_t* scales,
+                           int64_t ld_scales, void* stream);
+
+/* out (m, n) = a (m, k) * b (n, k)^T + bias (n, f32, or NULL), accumulated in f32 and rounded
+ * once to dtype (GQ_TYPE_F32, F16 or BF16).  a: e4m3 with one scale per 1 x 128 block,
+ * a_scales (m, ceil(k/128)); b: e4m3 with one scale per 128 x 128 block, b_scales
+ * (ceil(n/128), ceil(k/128)).  k a multiple of 32; m, n and k at most 2^31 - 1; every row of a
+ * and b starts on a 16-byte boundary, out and bias are aligned to their elements.  out must
+ * not overlap the inputs. */
+GQ_API int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64_t ld_a_scales,
+                         const uint8_t* b, int64_t ld_b, const uint8_t* b_scales, int64_t ld_b_scales,
+                         const float* bias, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,
+                         int64_t ld_out, void* stream);
+
 /* Host-buffer path: an opaque per-device session owning device staging memory, streams
  * and (on first use with pageable buffers) pinned bounce slots and host copy threads.
  * gq_convert_host copies each tensor's bytes host->device, converts and copies the results

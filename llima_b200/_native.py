@@ -24,6 +24,7 @@ EXPORTS = ("gq_version", "gq_strerror", "gq_last_cuda_error", "gq_kernel_errors"
            "gq_session_destroy", "gq_convert_host", "gq_convert_host_noalloc", "gq_embedding_rows",
            "gq_quantize_rows", "gq_modalix_layout", "gq_unpack_fields", "gq_remove_superblocks",
            "gq_convert_modalix", "gq_convert_modalix_batch",
+           "gq_convert_fp8", "gq_rms_norm_fp8", "gq_quantize_fp8", "gq_matmul_fp8",
            "gq_host_alloc", "gq_host_free", "gq_host_trim")
 
 
@@ -92,6 +93,10 @@ def _declare(lib):
         "gq_unpack_fields": ([I32, P, SZ, I64, P, P, P, P], ctypes.c_int),
         "gq_convert_modalix": ([ctypes.POINTER(Tensor), I64, P], ctypes.c_int),
         "gq_convert_modalix_batch": ([ctypes.POINTER(Tensor), P, I32, P], ctypes.c_int),
+        "gq_convert_fp8": ([ctypes.POINTER(Tensor), P, P], ctypes.c_int),
+        "gq_rms_norm_fp8": ([I32, P, I64, P, I64, P, ctypes.c_float, I64, I64, P, I64, P, I64, P, I64, P], ctypes.c_int),
+        "gq_quantize_fp8": ([I32, P, I64, P, I64, I64, I64, P, I64, P, I64, P], ctypes.c_int),
+        "gq_matmul_fp8": ([P, I64, P, I64, P, I64, P, I64, P, I64, I64, I64, I32, P, I64, P], ctypes.c_int),
         "gq_remove_superblocks": ([P, P, I32, I64, I32, I32, P, P, P], ctypes.c_int),
     }
     for name, (args, res) in sig.items():

@@ -126,6 +126,30 @@ int validate(const gq_tensor_t& t, int out_mask, TypeInfo* ti, int64_t* n_values
     return GQ_OK;
 }
 
+// ---- arguments of the 8-bit float entry points -------------------------------------------
+
+int float_bytes(int dtype) {
+    switch (dtype) {
+        case GQ_TYPE_F32: return 4;
+        case GQ_TYPE_F16:
+        case GQ_TYPE_BF16: return 2;
+        default: return 0;
+    }
+}
+
+constexpr int64_t kMaxStride = int64_t(1) << 38;   // the limit of a tensor map's byte strides is 2^40
+
+int rows_check(int64_t rows, int64_t cols) {
+    if (rows < 0 || cols < 0 || cols % 32 != 0) return GQ_ERR_SIZE;
+    if (rows > INT32_MAX || (cols != 0 && rows > INT64_MAX / 4 / cols)) return GQ_ERR_SIZE;
+    return GQ_OK;
+}
+
+// every row starts on a 16-byte boundary
+bool rows_aligned(const void* p, int64_t ld, int64_t rows, int elem_bytes) {
+    return aligned(p, 16) && (rows <= 1 || ld % (16 / elem_bytes) == 0);
+}
+
 gq::GqDesc make_desc(const gq_tensor_t& t, const TypeInfo& ti, int64_t n_units) {
     gq::GqDesc d{};
     d.src = static_cast<const uint8_t*>(t.src);
@@ -477,6 +501,132 @@ int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* codes, 
     if (!aligned(x, 16) || !aligned(codes, 4) || !aligned(scales_bf16, 2)) return GQ_ERR_ALIGN;
     return cuda_status(gq::launch_embed(GQ_TYPE_F32, true, reinterpret_cast<const uint8_t*>(x), rows, cols, cols * 4,
                                         1.0f, 1, codes, scales_bf16, nullptr, rows * cols * 4, stream));
+}
+
+// ---- block-scaled 8-bit floats -----------------------------------------------------------
+
+int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream) {
+    if (tensor == nullptr) return GQ_ERR_NULL;
+    const gq_tensor_t& t = *tensor;
+    TypeInfo ti;
+    int64_t nv = 0, nu = 0;
+    const int st = shape_check(t, &ti, &nv, &nu);
+    if (st != GQ_OK) return st;
+    if (t.cols % 32 != 0) return GQ_ERR_SIZE;
+    if (nv == 0) return GQ_OK;
+    if (t.src == nullptr || t.codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
+    if (!aligned(t.src, 16) || !aligned(t.codes, 16)) return GQ_ERR_ALIGN;
+    gq::GqFp8Weight p{};
+    p.src = static_cast<const uint8_t*>(t.src);
+    p.codes = static_cast<uint8_t*>(t.codes);
+    p.scales = scales;
+    p.rows = t.rows;
+    p.cols = t.cols;
+    p.row_bytes = t.cols / ti.unit_values * ti.unit_bytes;
+    p.src_bytes = nu * ti.unit_bytes;
+    p.scale_cols = (t.cols + 127) / 128;
+    if ((t.rows + 127) / 128 > INT32_MAX / p.scale_cols) return GQ_ERR_SIZE;
+    if (t.perm_heads > 0) {
+        if (t.rows / t.perm_heads > INT32_MAX) return GQ_ERR_SIZE;
+        p.head_dim = static_cast<int32_t>(t.rows / t.perm_heads);
+    }
+    return cuda_status(gq::launch_fp8_weight(t.type, p, stream));
+}
+
+int gq_rms_norm_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_residual,
+                    const float* weight, float eps, int64_t rows, int64_t cols, void* sum, int64_t ld_sum,
+                    uint8_t* codes, int64_t ld_codes, uint8_t* scales, int64_t ld_scales, void* stream) {
+    const int es = float_bytes(dtype);
+    if (es == 0) return GQ_ERR_TYPE;
+    int st = rows_check(rows, cols);
+    if (st != GQ_OK) return st;
+    if (ld_x < cols || ld_codes < cols || ld_scales < (cols + 127) / 128) return GQ_ERR_SIZE;
+    if (residual != nullptr && (ld_residual < cols || ld_sum < cols)) return GQ_ERR_SIZE;
+    if (rows == 0 || cols == 0) return GQ_OK;
+    if (x == nullptr || weight == nullptr || codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
+    if (residual != nullptr && sum == nullptr) return GQ_ERR_NULL;
+    if (!rows_aligned(x, ld_x, rows, es) || !rows_aligned(codes, ld_codes, rows, 1) || !aligned(weight, 16)) return GQ_ERR_ALIGN;
+    if (residual != nullptr && (!rows_aligned(residual, ld_residual, rows, es) || !rows_aligned(sum, ld_sum, rows, es)))
+        return GQ_ERR_ALIGN;
+    gq::GqFp8Rows p{};
+    p.x = static_cast<const uint8_t*>(x);
+    p.residual = static_cast<const uint8_t*>(residual);
+    p.weight = weight;
+    p.sum = static_cast<uint8_t*>(sum);
+    p.codes = codes;
+    p.scales = scales;
+    p.rows = rows;
+    p.cols = cols;
+    p.blocks = (cols + 127) / 128;
+    p.ld_x = ld_x;
+    p.ld_residual = ld_residual;
+    p.ld_sum = ld_sum;
+    p.ld_codes = ld_codes;
+    p.ld_scales = ld_scales;
+    p.eps = eps;
+    return cuda_status(gq::launch_fp8_rows(dtype, p, stream));
+}
+
+int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* gate, int64_t ld_gate, int64_t rows,
+                    int64_t cols, uint8_t* codes, int64_t ld_codes, uint8_t* scales, int64_t ld_scales, void* stream) {
+    const int es = float_bytes(dtype);
+    if (es == 0) return GQ_ERR_TYPE;
+    int st = rows_check(rows, cols);
+    if (st != GQ_OK) return st;
+    if (ld_x < cols || ld_codes < cols || ld_scales < (cols + 127) / 128) return GQ_ERR_SIZE;
+    if (gate != nullptr && ld_gate < cols) return GQ_ERR_SIZE;
+    if (rows == 0 || cols == 0) return GQ_OK;
+    if (x == nullptr || codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
+    if (!rows_aligned(x, ld_x, rows, es) || !rows_aligned(codes, ld_codes, rows, 1)) return GQ_ERR_ALIGN;
+    if (gate != nullptr && !rows_aligned(gate, ld_gate, rows, es)) return GQ_ERR_ALIGN;
+    gq::GqFp8Rows p{};
+    p.x = static_cast<const uint8_t*>(x);
+    p.gate = static_cast<const uint8_t*>(gate);
+    p.codes = codes;
+    p.scales = scales;
+    p.rows = rows;
+    p.cols = cols;
+    p.blocks = (cols + 127) / 128;
+    p.ld_x = ld_x;
+    p.ld_gate = ld_gate;
+    p.ld_codes = ld_codes;
+    p.ld_scales = ld_scales;
+    return cuda_status(gq::launch_fp8_rows(dtype, p, stream));
+}
+
+int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64_t ld_a_scales, const uint8_t* b,
+                  int64_t ld_b, const uint8_t* b_scales, int64_t ld_b_scales, const float* bias, int64_t m, int64_t n,
+                  int64_t k, int32_t dtype, void* out, int64_t ld_out, void* stream) {
+    const int es = float_bytes(dtype);
+    if (es == 0) return GQ_ERR_TYPE;
+    if (m < 0 || n < 0 || k < 0 || k % 32 != 0) return GQ_ERR_SIZE;
+    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return GQ_ERR_SIZE;
+    const int64_t kb = (k + 127) / 128;
+    if (ld_a < k || ld_b < k || ld_a_scales < kb || ld_b_scales < kb || ld_out < n) return GQ_ERR_SIZE;
+    if (ld_a > kMaxStride || ld_b > kMaxStride || ld_a_scales > kMaxStride || ld_b_scales > kMaxStride || ld_out > kMaxStride)
+        return GQ_ERR_SIZE;
+    if (m == 0 || n == 0) return GQ_OK;
+    if (out == nullptr) return GQ_ERR_NULL;
+    if (k != 0 && (a == nullptr || b == nullptr || a_scales == nullptr || b_scales == nullptr)) return GQ_ERR_NULL;
+    if (!aligned(out, es) || !aligned(bias, 4)) return GQ_ERR_ALIGN;
+    if (k != 0 && (!rows_aligned(a, ld_a, m, 1) || !rows_aligned(b, ld_b, n, 1))) return GQ_ERR_ALIGN;
+    gq::GqMatmul p{};
+    p.a = a;
+    p.a_scales = a_scales;
+    p.b = b;
+    p.b_scales = b_scales;
+    p.bias = bias;
+    p.out = static_cast<uint8_t*>(out);
+    p.m = m;
+    p.n = n;
+    p.k = k;
+    p.kb = kb;
+    p.ld_a = m > 1 ? ld_a : (k + 15) / 16 * 16;
+    p.ld_a_scales = ld_a_scales;
+    p.ld_b = n > 1 ? ld_b : (k + 15) / 16 * 16;
+    p.ld_b_scales = ld_b_scales;
+    p.ld_out = ld_out;
+    return cuda_status(gq::launch_matmul(dtype, p, stream));
 }
 
 // ---------------------------------------------------------------------------------------

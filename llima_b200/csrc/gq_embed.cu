@@ -14,6 +14,7 @@
 #include <cuda_bf16.h>
 #include <cuda_runtime.h>
 
+#include "gq_blocks.cuh"
 #include "gq_device.cuh"
 #include "gq_internal.h"
 
@@ -96,88 +97,12 @@ __device__ __forceinline__ void decode4(const uint8_t* row, int v, float out[4])
 
 __device__ __forceinline__ float to_bf16(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
 
-// ---- block view of a row, for the quantized formats ------------------------------------
-//
-// Block b of a row (16 values for Q6_K, 32 otherwise) as unsigned byte codes v (packed in
-// words, value j in byte j % 4 of word j / 4), an offset (the code is q = v - OFF) and the
-// constants of gguf-py's dequantize: x = RN(A * q), or RN(RN(A * q) - B) for Q4_K / Q5_K.
+// The formats whose rows are quantized block by block (gq_blocks.cuh).
 template <int TYPE>
-struct EmbBlock {
+struct EmbBlock : BlockView<TYPE> {
     static constexpr bool kOn = TYPE == GQ_TYPE_Q8_0 || TYPE == GQ_TYPE_Q4_0 || TYPE == GQ_TYPE_Q4_K ||
                                 TYPE == GQ_TYPE_Q5_K || TYPE == GQ_TYPE_Q6_K;
-    static constexpr int BV = TYPE == GQ_TYPE_Q6_K ? 16 : 32;
-    static constexpr int NW = BV / 4;
-    static constexpr int OFF = TYPE == GQ_TYPE_Q6_K ? 32 : (TYPE == GQ_TYPE_Q8_0 ? 128 : (TYPE == GQ_TYPE_Q4_0 ? 8 : 0));
-    static constexpr bool kSub = TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K;
 };
-
-template <int TYPE>
-__device__ __forceinline__ void decode_block(const uint8_t* row, int b, uint32_t (&w)[8], float& A, float& B) {
-    B = 0.0f;
-    if constexpr (TYPE == GQ_TYPE_Q6_K) {
-        // ql[128] | qh[64] | scales int8[16] | d; value 128h + 32g + j (ggml_quant.py:274-308)
-        const uint8_t* sp = row + 210 * (b >> 4);
-        const int kb = b & 15, h = kb >> 3, g = (kb >> 1) & 3, j0 = 16 * (kb & 1);
-        A = __fmul_rn(h2f(lds16(sp + 208)), static_cast<float>(static_cast<int8_t>(sp[192 + kb])));
-        const uint4 l = lds128_align2(sp + 64 * h + 32 * (g & 1) + j0);
-        const uint4 q = lds128_align2(sp + 128 + 32 * h + j0);
-        const uint32_t lw[4] = {l.x, l.y, l.z, l.w}, hw[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = ((lw[i] >> (4 * (g >> 1))) & 0x0F0F0F0Fu) | (((hw[i] >> (2 * g)) & 0x03030303u) << 4);
-    } else if constexpr (TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K) {
-        // d, dmin | scales[12] | (qh[32]) | qs[128]; block k: nibble k & 1 of qs[32(k/2) + j]
-        constexpr bool Q5 = TYPE == GQ_TYPE_Q5_K;
-        const uint8_t* sp = row + (Q5 ? 176 : 144) * (b >> 3);
-        const int k = b & 7, g = k >> 1;
-        int sc, mn;
-        if (k < 4) {
-            sc = sp[4 + k] & 63;
-            mn = sp[8 + k] & 63;
-        } else {
-            sc = (sp[12 + k - 4] & 0xF) | ((sp[4 + k - 4] >> 6) << 4);
-            mn = (sp[12 + k - 4] >> 4) | ((sp[8 + k - 4] >> 6) << 4);
-        }
-        A = __fmul_rn(h2f(lds16(sp)), static_cast<float>(sc));
-        B = __fmul_rn(h2f(lds16(sp + 2)), static_cast<float>(mn));
-        const uint8_t* qp = sp + (Q5 ? 48 : 16) + 32 * g;
-        const uint4 a0 = lds128_align2(qp), a1 = lds128_align2(qp + 16);
-        const uint32_t x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = (x[i] >> (4 * (k & 1))) & 0x0F0F0F0Fu;
-        if constexpr (Q5) {
-            const uint4 c0 = lds128_align2(sp + 16), c1 = lds128_align2(sp + 32);
-            const uint32_t hb[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-#pragma unroll
-            for (int i = 0; i < 8; ++i) w[i] |= ((hb[i] >> k) & 0x01010101u) << 4;
-        }
-    } else if constexpr (TYPE == GQ_TYPE_Q8_0) {
-        // d | int8[32]: the codes biased by 128 to unsigned bytes
-        const uint8_t* bp = row + 34 * b;
-        A = h2f(lds16(bp));
-        const uint4 a0 = lds128_align2(bp + 2), a1 = lds128_align2(bp + 18);
-        const uint32_t x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = x[i] ^ 0x80808080u;
-    } else {   // Q4_0: d | nibbles[16]; value j < 16 low nibble of byte j, else high of j - 16
-        const uint8_t* bp = row + 18 * b;
-        A = h2f(lds16(bp));
-        const uint4 a0 = lds128_align2(bp + 2);
-        const uint32_t x[4] = {a0.x, a0.y, a0.z, a0.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            w[i] = x[i] & 0x0F0F0F0Fu;
-            w[4 + i] = (x[i] >> 4) & 0x0F0F0F0Fu;
-        }
-    }
-}
-
-// x of code q, as gguf-py computes it (Q8_0: x * d, the same product)
-template <int TYPE>
-__device__ __forceinline__ float block_value(float A, float B, int q) {
-    const float p = __fmul_rn(A, static_cast<float>(q));
-    return EmbBlock<TYPE>::kSub ? __fsub_rn(p, B) : p;
-}
 
 // code of y = bf16(x * embed_scale) for the row step: clip(rint(y / step), -127, 127).
 // fast (step a normal number): y * (1/step) is within 2^-15 of y / step for every |y| <=

@@ -1,0 +1,48 @@
+// e4m3 codes and power-of-two (E8M0) block scales.
+//
+// A block's scale is 2^e with the smallest e >= -127 such that its largest finite magnitude
+// is at most 448 * 2^e (448 = 1.75 * 2^8 is the largest e4m3 value); e = 0 for an all-zero
+// block.  Dividing by a power of two is exact, so a code is its value rounded once, and
+// dequantization is exact.  e4m3 keeps four significant bits whatever the scale, so a finer
+// scale than a power of two would gain nothing but part of the last binade; this form is the
+// one the tensor cores multiply by themselves.
+#pragma once
+
+#include "gq_device.cuh"
+
+namespace gq {
+
+constexpr int kFp8Block = 128;
+constexpr uint32_t kInfBits = 0x7F800000u;
+
+// |x| bits where x is finite, else 0
+__device__ __forceinline__ uint32_t finite_abs(float x) {
+    const uint32_t b = __float_as_uint(x) & 0x7FFFFFFFu;
+    return b < kInfBits ? b : 0u;
+}
+
+// The stored scale byte e + 127 for the bit pattern of the block's largest finite |x|:
+// amax = 1.f * 2^(E - 127) <= 1.75 * 2^(8 + e) <=> e >= E - 135 + (f > 0.75).
+__device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
+    if (amax_bits == 0) return 127u;
+    const int e = static_cast<int>(amax_bits >> 23) - 8 + ((amax_bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+    return static_cast<uint32_t>(max(e, 0));
+}
+
+// 2^-e of a scale byte (0..247), a normal number
+__device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
+
+// Two values already divided by the scale to two codes (x in the low byte), round to nearest
+// even.  The conversion saturates, which no finite value here needs (|x| <= 448).
+__device__ __forceinline__ uint32_t e4m3x2(float x, float y) {
+    uint16_t r;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(x), "f"(y));
+    return r;
+}
+
+// The same for any value: one that is not finite becomes the NaN code
+__device__ __forceinline__ float nan_unless_finite(float x) {
+    return (__float_as_uint(x) & 0x7FFFFFFFu) < kInfBits ? x : __uint_as_float(0x7FFFFFFFu);
+}
+
+}  // namespace gq

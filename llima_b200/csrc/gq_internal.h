@@ -95,4 +95,52 @@ int launch_fields(int type, const uint8_t* src, int64_t n_units, float* sup, int
 int launch_superblocks(const float* sup, const void* blk, int blk_bytes, int64_t n_super, int nb, int k,
                        uint16_t* out_f16, float* out_f32, void* stream);
 
+
+// A GGUF tensor to e4m3 codes (rows, cols) and one E8M0 scale per 128 x 128 block
+// (ceil(rows / 128), scale_cols).
+struct GqFp8Weight {
+    const uint8_t* src;
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t rows, cols;
+    int64_t row_bytes, src_bytes;   // of the GGUF tensor
+    int64_t scale_cols;
+    int32_t head_dim;         // > 0: llama q/k head permutation with heads of this size
+    uint32_t n_col_tiles;     // set by the launch
+};
+
+// Activations (rows, cols) to e4m3 codes and one E8M0 scale per 1 x 128 block.  weight set:
+// RMS norm (with the residual's addition when residual is set); gate set: silu(gate) * x.
+// Strides in elements; the last of each row is 1.
+struct GqFp8Rows {
+    const uint8_t* x;
+    const uint8_t* gate;
+    const uint8_t* residual;
+    const float* weight;
+    uint8_t* sum;
+    uint8_t* codes;
+    uint8_t* scales;
+    int64_t rows, cols, blocks;   // blocks = ceil(cols / 128)
+    int64_t ld_x, ld_gate, ld_residual, ld_sum, ld_codes, ld_scales;
+    float eps;
+};
+
+// out (m, n) = a (m, k) b (n, k)^T + bias (n): e4m3 operands, a with a scale per 1 x 128
+// block, b with one per 128 x 128.
+struct GqMatmul {
+    const uint8_t* a;
+    const uint8_t* a_scales;
+    const uint8_t* b;
+    const uint8_t* b_scales;
+    const float* bias;
+    uint8_t* out;
+    int64_t m, n, k, kb;          // kb = ceil(k / 128)
+    int64_t ld_a, ld_a_scales, ld_b, ld_b_scales, ld_out;
+};
+
+// implemented in gq_fp8.cu and gq_matmul.cu
+int launch_fp8_weight(int type, GqFp8Weight& p, void* stream);
+int launch_fp8_rows(int dtype, const GqFp8Rows& p, void* stream);
+int launch_matmul(int dtype, const GqMatmul& p, void* stream);
+
 }  // namespace gq

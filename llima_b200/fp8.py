@@ -1,0 +1,309 @@
+"""Block-scaled 8-bit floats: a GGUF file's projections on the GPU itself.
+
+The reference prepares integer weights and leaves the products to the Modalix accelerator
+(``ModelGraph.linear``, ``sima_lmm/model/model_graph.py:351-403``).  Here the same GGUF
+tensors become e4m3 weights that the B200's tensor cores multiply directly, with the two
+operators that feed them:
+
+* ``convert_fp8_device`` / ``fp8_from_gguf``: a GGUF tensor to e4m3 codes with one
+  power-of-two scale per 128 x 128 block (``Fp8Weight``);
+* ``rms_norm_fp8``: RMS norm, with the residual's addition, to e4m3 rows with one scale per
+  1 x 128 block (``Fp8Rows``);
+* ``quantize_fp8``: rows, or silu(gate) * rows, quantized the same way;
+* ``matmul_fp8``: ``Fp8Rows`` times ``Fp8Weight``, for one token as for a long prompt;
+* ``Fp8Linear`` and ``Fp8FeedForward``: a projection, and a layer's gated feed-forward block,
+  from a GGUF file's tensors.
+
+Scales are ``float8_e8m0fnu``: 2^e with the smallest e >= -127 for which the block's largest
+finite magnitude is at most 448 * 2^e.  A value that is not finite becomes the NaN code.
+Row counts are free; column counts are multiples of 32, as every quantized GGUF row's are.
+
+Work is enqueued on the current stream of the operands' device, whichever device is
+current, and no call waits for it.
+"""
+from __future__ import annotations
+
+import ctypes
+from typing import NamedTuple
+
+import numpy as np
+import torch
+
+from . import _native as N
+from .formats import FORMATS
+
+__all__ = ["Fp8Rows", "Fp8Weight", "convert_fp8_device", "fp8_from_gguf", "rms_norm_fp8", "quantize_fp8",
+           "matmul_fp8", "Fp8Linear", "Fp8FeedForward"]
+
+BLOCK = 128
+E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_TYPE_IDS = {torch.float32: FORMATS["F32"].type_id, torch.float16: FORMATS["F16"].type_id,
+             torch.bfloat16: FORMATS["BF16"].type_id}
+
+
+class Fp8Rows(NamedTuple):
+    """Activations: codes (rows, cols) float8_e4m3fn and scales (rows, ceil(cols / 128))
+    float8_e8m0fnu."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class Fp8Weight(NamedTuple):
+    """Weights: codes (rows, cols) float8_e4m3fn, rows = output channels, and scales
+    (ceil(rows / 128), ceil(cols / 128)) float8_e8m0fnu."""
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+
+class _On:
+    """The device of a call made current, and its current stream."""
+    __slots__ = ("guard", "stream")
+
+    def __init__(self, device: torch.device):
+        self.guard = None
+        if device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
+def _matrix(t: torch.Tensor, name: str, dtype, device: torch.device | None, rows: int | None = None,
+            cols: int | None = None) -> int:
+    """Checks a 2-D CUDA operand whose rows are consecutive elements; returns its row stride."""
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if t.dim() != 2:
+        raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
+    r, c = t.shape
+    if (rows is not None and r != rows) or (cols is not None and c != cols):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
+                         f"{(r if rows is None else rows, c if cols is None else cols)}")
+    s0, s1 = t.stride()
+    if c > 1 and s1 != 1:
+        raise ValueError(f"the elements of a row of {name} must be consecutive (strides {t.stride()})")
+    if r <= 1:
+        return c
+    if s0 < c:
+        raise ValueError(f"the rows of {name} overlap (strides {t.stride()})")
+    return s0
+
+
+def _float_rows(x: torch.Tensor, name: str) -> int:
+    if x.dtype not in _TYPE_IDS:
+        raise TypeError(f"{name} must be float32, float16 or bfloat16, not {x.dtype}")
+    if x.dim() == 2 and x.shape[1] % 32:
+        raise ValueError(f"{name} has {x.shape[1]} columns: a multiple of 32 is needed")
+    return _matrix(x, name, x.dtype, None)
+
+
+def _rows_out(rows: int, cols: int, device, out: Fp8Rows | None):
+    blocks = (cols + BLOCK - 1) // BLOCK
+    if out is None:
+        return Fp8Rows(torch.empty((rows, cols), dtype=E4M3, device=device),
+                       torch.empty((rows, blocks), dtype=E8M0, device=device)), cols, blocks
+    ld = _matrix(out.codes, "out.codes", E4M3, device, rows, cols)
+    return out, ld, _matrix(out.scales, "out.scales", E8M0, device, rows, blocks)
+
+
+def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads: int = 0,
+                       out: Fp8Weight | None = None) -> Fp8Weight:
+    """GGUF bytes already on the GPU (uint8, 16-byte aligned) -> ``Fp8Weight``.  The values
+    quantized are those of the f32 conversion, bit for bit; heads > 0 applies the llama q/k
+    row permutation (``GgufModel._permute_qk_proj``, gguf_conversion.py:314-332)."""
+    f = FORMATS[fmt]
+    if src.dtype != torch.uint8 or not src.is_cuda or not src.is_contiguous():
+        raise TypeError("src must be a contiguous CUDA uint8 tensor of GGUF bytes")
+    shape = ((rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
+    if out is None:
+        if rows < 0 or cols < 0:
+            raise ValueError(f"negative shape ({rows}, {cols})")
+        out = Fp8Weight(torch.empty((rows, cols), dtype=E4M3, device=src.device),
+                        torch.empty(shape, dtype=E8M0, device=src.device))
+    else:
+        _matrix(out.codes, "out.codes", E4M3, src.device, rows, cols)
+        _matrix(out.scales, "out.scales", E8M0, src.device, *shape)
+        if not out.codes.is_contiguous() or not out.scales.is_contiguous():
+            raise ValueError("out must be contiguous")
+    t = N.Tensor(type=f.type_id, perm_heads=heads, rows=rows, cols=cols, src=src.data_ptr(), src_bytes=src.numel(),
+                 codes=out.codes.data_ptr())
+    with _On(src.device) as stream:
+        N.check(N.lib().gq_convert_fp8(ctypes.byref(t), out.scales.data_ptr(), stream), "gq_convert_fp8")
+    return out
+
+
+def fp8_from_gguf(gguf_tensor, heads: int = 0, device=None) -> Fp8Weight:
+    """``Fp8Weight`` of one reader tensor (rows = output channels).  ``device``: a CUDA
+    device, the current one by default."""
+    from .gguf_conversion import _type_name
+    fmt = _type_name(gguf_tensor.tensor_type)
+    if fmt not in FORMATS:
+        raise NotImplementedError(f"GGML type {fmt} is not handled by the B200 GGUF path")
+    shape = tuple(int(x) for x in gguf_tensor.shape[::-1])
+    if len(shape) != 2:
+        raise ValueError(f"{gguf_tensor.name}: a weight has two dimensions, not {len(shape)}")
+    raw = np.ascontiguousarray(gguf_tensor.data).reshape(-1).view(np.uint8)
+    src = torch.from_numpy(raw if raw.flags.writeable else raw.copy()).to("cuda" if device is None else device)
+    return convert_fp8_device(fmt, src, *shape, heads)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, residual: torch.Tensor | None = None,
+                 sum_out: torch.Tensor | None = None, out: Fp8Rows | None = None):
+    """RMS norm of the rows of ``x`` (rows, cols), quantized: ``Fp8Rows`` of
+    h / sqrt(mean(h^2) + eps) * weight, weight float32 (cols).  With ``residual`` (of x's
+    type and shape), h = x + residual rounded to that type and (``Fp8Rows``, h) is returned;
+    ``sum_out`` receives h and may be ``residual`` or ``x`` itself."""
+    ld_x = _float_rows(x, "x")
+    rows, cols = x.shape
+    dev = x.device
+    if weight.dtype != torch.float32 or weight.shape != (cols,) or weight.device != dev or not weight.is_contiguous():
+        raise ValueError(f"weight must be a contiguous float32 tensor of {cols} values on {dev}")
+    ld_r = ld_s = 0
+    if residual is not None:
+        ld_r = _matrix(residual, "residual", x.dtype, dev, rows, cols)
+        if sum_out is None:
+            sum_out = torch.empty((rows, cols), dtype=x.dtype, device=dev)
+        ld_s = _matrix(sum_out, "sum_out", x.dtype, dev, rows, cols)
+    elif sum_out is not None:
+        raise ValueError("sum_out without residual")
+    out, ld_c, ld_sc = _rows_out(rows, cols, dev, out)
+    with _On(dev) as stream:
+        N.check(N.lib().gq_rms_norm_fp8(_TYPE_IDS[x.dtype], x.data_ptr(), ld_x,
+                                        None if residual is None else residual.data_ptr(), ld_r, weight.data_ptr(), eps,
+                                        rows, cols, None if residual is None else sum_out.data_ptr(), ld_s,
+                                        out.codes.data_ptr(), ld_c, out.scales.data_ptr(), ld_sc, stream),
+                "gq_rms_norm_fp8")
+    return out if residual is None else (out, sum_out)
+
+
+def quantize_fp8(x: torch.Tensor, gate: torch.Tensor | None = None, out: Fp8Rows | None = None) -> Fp8Rows:
+    """Rows of ``x`` (rows, cols), or silu(gate) * x with ``gate`` of x's type and shape, as
+    ``Fp8Rows``.  Both may be column ranges of one wider tensor, as a fused gate and up
+    product leaves them."""
+    ld_x = _float_rows(x, "x")
+    rows, cols = x.shape
+    ld_g = 0 if gate is None else _matrix(gate, "gate", x.dtype, x.device, rows, cols)
+    out, ld_c, ld_sc = _rows_out(rows, cols, x.device, out)
+    with _On(x.device) as stream:
+        N.check(N.lib().gq_quantize_fp8(_TYPE_IDS[x.dtype], x.data_ptr(), ld_x, None if gate is None else gate.data_ptr(),
+                                        ld_g, rows, cols, out.codes.data_ptr(), ld_c, out.scales.data_ptr(), ld_sc,
+                                        stream), "gq_quantize_fp8")
+    return out
+
+
+def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """a (m, k) times w (n, k) transposed, plus ``bias`` (n, float32): (m, n) of ``dtype``
+    (bfloat16, float16 or float32; that of ``out`` when given), accumulated in float32 and
+    rounded once.  ``out`` must not overlap the operands."""
+    codes, scales = a
+    w_codes, w_scales = w
+    dev = codes.device
+    ld_a = _matrix(codes, "a.codes", E4M3, None)
+    m, k = codes.shape
+    if k % 32:
+        raise ValueError(f"a.codes has {k} columns: a multiple of 32 is needed")
+    blocks = (k + BLOCK - 1) // BLOCK
+    ld_sa = _matrix(scales, "a.scales", E8M0, dev, m, blocks)
+    ld_b = _matrix(w_codes, "w.codes", E4M3, dev, None, k)
+    n = w_codes.shape[0]
+    ld_sb = _matrix(w_scales, "w.scales", E8M0, dev, (n + BLOCK - 1) // BLOCK, blocks)
+    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != dev
+                             or not bias.is_contiguous()):
+        raise ValueError(f"bias must be a contiguous float32 tensor of {n} values on {dev}")
+    if out is None:
+        if dtype not in _TYPE_IDS:
+            raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
+        out = torch.empty((m, n), dtype=dtype, device=dev)
+        ld_o = n
+    else:
+        if out.dtype not in _TYPE_IDS:
+            raise TypeError(f"out must be float32, float16 or bfloat16, not {out.dtype}")
+        ld_o = _matrix(out, "out", out.dtype, dev, m, n)
+    with _On(dev) as stream:
+        N.check(N.lib().gq_matmul_fp8(codes.data_ptr(), ld_a, scales.data_ptr(), ld_sa, w_codes.data_ptr(), ld_b,
+                                      w_scales.data_ptr(), ld_sb, None if bias is None else bias.data_ptr(), m, n, k,
+                                      _TYPE_IDS[out.dtype], out.data_ptr(), ld_o, stream), "gq_matmul_fp8")
+    return out
+
+
+class Fp8Linear:
+    """One projection: ``Fp8Weight`` and an optional float32 bias."""
+
+    def __init__(self, weight: Fp8Weight, bias: torch.Tensor | None = None):
+        self.weight = weight
+        self.bias = bias
+
+    @classmethod
+    def from_gguf(cls, gguf_tensor, bias_tensor=None, heads: int = 0, device=None) -> "Fp8Linear":
+        """From a reader's weight tensor and, where the model has one, its bias tensor;
+        heads > 0 applies the llama q/k row permutation to both."""
+        weight = fp8_from_gguf(gguf_tensor, heads, device)
+        bias = None
+        if bias_tensor is not None:
+            from .gguf_conversion import load_tensor
+            b = np.array(load_tensor(bias_tensor, True, heads)[1], dtype=np.float32).reshape(-1)
+            bias = torch.from_numpy(b).to(weight.codes.device)
+        return cls(weight, bias)
+
+    def __call__(self, x: Fp8Rows | torch.Tensor, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        """x as ``Fp8Rows``, or float rows that are quantized first."""
+        if not isinstance(x, Fp8Rows):
+            x = quantize_fp8(x)
+        return matmul_fp8(x, self.weight, self.bias, dtype)
+
+
+class Fp8FeedForward:
+    """A layer's gated feed-forward block: x + residual -> RMS norm -> gate and up products ->
+    silu(gate) * up -> down product, every product on e4m3 operands.  The gate and up weights
+    sit in one tensor and are one product."""
+
+    def __init__(self, norm: torch.Tensor, gate_up: Fp8Weight, down: Fp8Weight, eps: float = 1e-5):
+        self.norm, self.gate_up, self.down, self.eps = norm, gate_up, down, eps
+
+    @classmethod
+    def from_gguf(cls, reader, layer: int, device=None) -> "Fp8FeedForward":
+        """From a ``gguf.GGUFReader`` (or a path) by the tensors' GGUF names: ``blk.N.ffn_norm``,
+        ``ffn_gate``, ``ffn_up`` and ``ffn_down``; the epsilon from the file's metadata."""
+        if not hasattr(reader, "tensors"):
+            from gguf import GGUFReader
+            reader = GGUFReader(reader)
+        from .gguf_conversion import _type_name, load_tensor
+        names = {t.name: t for t in reader.tensors}
+        norm, gate, up, down = (names[f"blk.{layer}.ffn_{part}.weight"] for part in ("norm", "gate", "up", "down"))
+        arch = reader.fields["general.architecture"].contents()
+        eps = float(reader.fields[f"{arch}.attention.layer_norm_rms_epsilon"].contents())
+        dev = torch.device("cuda" if device is None else device)
+        rows, cols = (int(x) for x in gate.shape[::-1])
+        if tuple(up.shape) != tuple(gate.shape):
+            raise ValueError(f"gate and up weights differ in shape: {tuple(gate.shape)}, {tuple(up.shape)}")
+        if rows % BLOCK:
+            raise ValueError(f"{rows} feed-forward channels: a multiple of {BLOCK} is needed to keep the gate and up "
+                             "weights in one tensor")
+        both = Fp8Weight(torch.empty((2 * rows, cols), dtype=E4M3, device=dev),
+                         torch.empty((2 * rows // BLOCK, -(-cols // BLOCK)), dtype=E8M0, device=dev))
+        for i, t in enumerate((gate, up)):
+            part = slice(i * rows, (i + 1) * rows), slice(i * rows // BLOCK, (i + 1) * rows // BLOCK)
+            raw = torch.from_numpy(np.array(t.data).reshape(-1).view(np.uint8)).to(dev)
+            convert_fp8_device(_type_name(t.tensor_type), raw, rows, cols,
+                               out=Fp8Weight(both.codes[part[0]], both.scales[part[1]]))
+        w = torch.from_numpy(np.array(load_tensor(norm, True)[1], dtype=np.float32).reshape(-1)).to(dev)
+        return cls(w, both, fp8_from_gguf(down, device=dev), eps)
+
+    def __call__(self, x: torch.Tensor, residual: torch.Tensor):
+        """x and residual (rows, hidden) -> (the block's output, the residual that it is to be
+        added to: x + residual), both of x's type."""
+        q, h = rms_norm_fp8(x, self.norm, self.eps, residual=residual)
+        both = matmul_fp8(q, self.gate_up, dtype=x.dtype)
+        half = both.shape[1] // 2
+        return matmul_fp8(quantize_fp8(both[:, half:], gate=both[:, :half]), self.down, dtype=x.dtype), h

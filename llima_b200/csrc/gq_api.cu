@@ -228,7 +228,12 @@ int gq_kernel_errors(int32_t device, int32_t clear, uint32_t* flags) {
     *flags = 0;
     const DeviceScope scope(device);
     if (scope.status() != GQ_OK) return scope.status();
-    return cuda_status(gq::kernel_errors(clear != 0, flags));
+    uint32_t more = 0;
+    const int st = cuda_status(gq::kernel_errors(clear != 0, flags));
+    if (st != GQ_OK) return st;
+    const int sm = cuda_status(gq::matmul_errors(clear != 0, &more));
+    *flags |= more;
+    return sm;
 }
 
 int gq_query(int32_t type, int64_t rows, int64_t cols, gq_layout_t* out) {

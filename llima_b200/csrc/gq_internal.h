@@ -142,5 +142,6 @@ struct GqMatmul {
 int launch_fp8_weight(int type, GqFp8Weight& p, void* stream);
 int launch_fp8_rows(int dtype, const GqFp8Rows& p, void* stream);
 int launch_matmul(int dtype, const GqMatmul& p, void* stream);
+int matmul_errors(bool clear, uint32_t* flags);   // as kernel_errors, of the product kernels
 
 }  // namespace gq

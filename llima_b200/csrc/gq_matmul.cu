@@ -1,18 +1,29 @@
-// out = a b^T (+ bias) for block-scaled e4m3 operands.
+// out = a b^T (+ bias) for block-scaled e4m3 operands, on the tensor cores.
 //
-// One CTA per 64 x 64 tile of the output, 4 x 4 values per thread; 32 columns of both
-// operands at a time are widened to f32 in shared memory.  Each 128-column block's products
-// are summed on their own and join the total times both scales.
+// The matrix instruction (tcgen05.mma, kind mxf8f6f4) takes one E8M0 scale per row and 32
+// columns and multiplies by it itself, so a 1 x 128 or 128 x 128 block's scale is the same
+// byte for four instructions and the sum over all of k stays in tensor memory.
+//
+// gq_matmul_narrow: the weights' 128 rows are the instruction's M and the tokens its N, so
+// that a few tokens cost a narrow instruction and not a padded one.  What bounds it is the
+// weights' traffic: a CTA streams its 128 rows through a ring of 128-column tiles.  Where
+// there are too few row tiles for the SMs, a cluster of 2 to 8 CTAs splits k and adds the
+// partial sums over distributed shared memory in a fixed order.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
-#include "gq_device.cuh"
+#include <mutex>
+
 #include "gq_internal.h"
+#include "gq_tcgen05.cuh"
 
 namespace gq {
 namespace {
+
+// Sticky error flags of this device's product kernels (kErrWaitTimeout).
+__device__ unsigned int gq_matmul_errors;
 
 template <class T>
 __device__ __forceinline__ T out_cast(float x);
@@ -23,56 +34,297 @@ __device__ __forceinline__ __half out_cast<__half>(float x) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 out_cast<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
 
-__device__ __forceinline__ float e8m0_value(uint32_t b) {
-    return b == 255u ? __uint_as_float(0x7FFFFFFFu) : __uint_as_float(b == 0 ? 0x00400000u : b << 23);
+// Four values to one row of the output, as one store where the address allows it
+template <class T>
+__device__ __forceinline__ void store4(T* out, const float (&v)[4], int64_t left) {
+    if (left >= 4 && (reinterpret_cast<uintptr_t>(out) & (4 * sizeof(T) - 1)) == 0) {
+        if constexpr (sizeof(T) == 4) {
+            stg128f(reinterpret_cast<float*>(out), v[0], v[1], v[2], v[3]);
+        } else {
+            T c[4] = {out_cast<T>(v[0]), out_cast<T>(v[1]), out_cast<T>(v[2]), out_cast<T>(v[3])};
+            uint2 w;
+            memcpy(&w, c, sizeof(w));
+            st_global(reinterpret_cast<uint2*>(out), w);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (i < left) out[i] = out_cast<T>(v[i]);
+    }
 }
 
-template <class T>
-__global__ void __launch_bounds__(256) gq_matmul_kernel(const GqMatmul p) {
-    __shared__ float sa[64][33], sb[64][33];
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-    const int64_t tiles_n = (p.n + 63) / 64;
-    const int64_t m0 = blockIdx.x / tiles_n * 64, n0 = blockIdx.x % tiles_n * 64;
-    float total[4][4] = {}, part[4][4] = {};
-    for (int64_t k0 = 0; k0 < p.k; k0 += 32) {
-        const int r = tid >> 2, c = 8 * (tid & 3);
-        for (int i = 0; i < 8; ++i) {
-            __nv_fp8_e4m3 x, y;
-            x.__x = m0 + r < p.m ? p.a[(m0 + r) * p.ld_a + k0 + c + i] : 0;
-            y.__x = n0 + r < p.n ? p.b[(n0 + r) * p.ld_b + k0 + c + i] : 0;
-            sa[r][c + i] = static_cast<float>(x);
-            sb[r][c + i] = static_cast<float>(y);
+// Four consecutive scale bytes from block kb on as a word; blocks from `blocks` on read as 1
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int64_t kb, int64_t blocks) {
+    const uint8_t* s = row + kb;
+    if (kb + 4 <= blocks && (reinterpret_cast<uintptr_t>(s) & 3) == 0) return *reinterpret_cast<const uint32_t*>(s);
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w |= (kb + i < blocks ? static_cast<uint32_t>(s[i]) : 127u) << (8 * i);
+    return w;
+}
+
+constexpr int kTileK = 128;
+constexpr int kSfSlots = 4;      // groups of four 128-column blocks whose scales are staged
+
+template <int BN>
+struct Narrow {
+    static constexpr int kThreads = 192;
+    static constexpr int kStageBytes = 128 * kTileK + BN * kTileK;
+    static constexpr int kStages = BN <= 32 ? 5 : BN == 64 ? 4 : 3;
+    static constexpr int kSfBytes = 1024;                          // 512 for each operand
+    static constexpr int kBars = 2 * kStages + 2 * kSfSlots + 1;
+    static constexpr int kRing = kStages * kStageBytes;            // reused for the f32 sums
+    static constexpr int kUsed = 1024 + kRing + kSfSlots * kSfBytes + 8 * kBars + 16;
+    static constexpr int kCols = BN + 8 * kSfSlots <= 64 ? 64 : BN + 8 * kSfSlots <= 128 ? 128 : 256;
+    // CTAs that share an SM must find room in its 512 columns of tensor memory together, so
+    // that none waits for another's (in a cluster that could be a circle): shared memory is
+    // taken in the same proportion, 228 KB for 512 columns.
+    static constexpr int kLeast = kCols * 228 * 2 - 1024;
+    static constexpr int kSmem = kUsed > kLeast ? kUsed : kLeast;
+    static_assert(kRing >= BN * 128 * 4, "the sums fit the ring");
+    static_assert(kSmem <= 227 * 1024, "one CTA's shared memory");
+};
+
+template <int BN, class T>
+__global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const __grid_constant__ CUtensorMap map_b,
+                                                                         const __grid_constant__ CUtensorMap map_a,
+                                                                         const GqMatmul p, const int split) {
+    using C = Narrow<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
+    uint8_t* const smem = smem_raw + (base - smem_u32addr(smem_raw));
+    const uint32_t sf = base + C::kRing, bars = sf + kSfSlots * C::kSfBytes, slot = bars + 8 * C::kBars;
+    const auto full = [&](int s) { return bars + 8 * s; };
+    const auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
+    const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
+    const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + kSfSlots + s); };
+    const uint32_t done = bars + 8 * (C::kBars - 1);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+
+    const uint32_t rank = split > 1 ? tc::cluster_rank() : 0;
+    const int64_t tile = blockIdx.x / split;
+    const int64_t m_tiles = (p.m + BN - 1) / BN;
+    const int64_t m0 = tile % m_tiles * BN, n0 = tile / m_tiles * 128;
+    const int kb0 = static_cast<int>(p.kb * rank / split), kb1 = static_cast<int>(p.kb * (rank + 1) / split);
+    const int blocks = kb1 - kb0;
+
+    if (warp == 5) tc::tmem_alloc<C::kCols>(slot);
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            tc::init(full(s), 1);
+            tc::init(empty(s), 1);
         }
-        __syncthreads();
-        for (int k = 0; k < 32; ++k)
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) part[i][j] = __fmaf_rn(sa[4 * ty + i][k], sb[tx + 16 * j][k], part[i][j]);
-        __syncthreads();
-        if ((k0 & 127) == 96 || k0 + 32 >= p.k) {
-            for (int i = 0; i < 4; ++i)
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t m = m0 + 4 * ty + i, n = n0 + tx + 16 * j;
-                    if (m < p.m && n < p.n)
-                        total[i][j] += part[i][j] * e8m0_value(p.a_scales[m * p.ld_a_scales + k0 / 128]) *
-                                       e8m0_value(p.b_scales[n / 128 * p.ld_b_scales + k0 / 128]);
-                    part[i][j] = 0.0f;
+        for (int s = 0; s < kSfSlots; ++s) {
+            tc::init(sf_full(s), 1);
+            tc::init(sf_empty(s), 1);
+        }
+        tc::init(done, 1);
+        mbar_init_fence();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::fence_after();
+    const uint32_t tmem = lds_u32(slot);
+
+    bool ok = true;
+    if (warp == 4) {
+        if (lane == 0) {
+            tc::prefetch_map(&map_b);
+            tc::prefetch_map(&map_a);
+            int issued = 0;
+            for (int i = 0; i < blocks; ++i) {
+                const int s = i % C::kStages, round = i / C::kStages;
+                if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+                tc::arrive_expect(full(s), C::kStageBytes);
+                const uint32_t at = base + s * C::kStageBytes;
+                tc::load_tile(at, &map_b, (kb0 + i) * kTileK, static_cast<int>(n0), full(s));
+                tc::load_tile(at + 128 * kTileK, &map_a, (kb0 + i) * kTileK, static_cast<int>(m0), full(s));
+                issued = i + 1;
+            }
+            // nothing of this CTA is in flight when it ends, also after a wait that gave up
+            if (!ok)
+                for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
+        }
+    } else if (warp == 5) {
+        if (lane == 0) {
+            for (int i = 0; i < blocks; ++i) {
+                const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
+                const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
+                if (i % 4 == 0) {
+                    if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
+                    tc::fence_after();
+                    tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
+                    tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
                 }
+                if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
+                tc::fence_after();
+                const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
+                const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
+                const uint32_t idesc = tc::instruction<128, BN>(i % 4);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) tc::mma(tmem, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
+                tc::commit(empty(s));
+                if (i % 4 == 3 || i + 1 == blocks) tc::commit(sf_empty(q));
+            }
+            tc::commit(done);
+        }
+    } else if (warp == 2) {
+        // scales: the weights' byte is the same for all 128 rows of the tile
+        const uint8_t* wrow = p.b_scales + (n0 >> 7) * p.ld_b_scales;
+        for (int i = 0; i < blocks; i += 4) {
+            const int g = i / 4, q = g % kSfSlots, round = g / kSfSlots;
+            const uint32_t w = scale_word(wrow, kb0 + i, p.kb);
+            uint32_t x[(BN + 31) / 32];
+#pragma unroll
+            for (int j = 0; j < (BN + 31) / 32; ++j) {
+                const int64_t m = m0 + 32 * j + lane;
+                x[j] = m < p.m ? scale_word(p.a_scales + m * p.ld_a_scales, kb0 + i, p.kb) : 0x7F7F7F7Fu;
+            }
+            if (round > 0 && !(ok = tc::wait(sf_empty(q), (round - 1) & 1))) break;
+            sts(sf + q * C::kSfBytes + 16 * lane, make_uint4(w, w, w, w));
+#pragma unroll
+            for (int j = 0; j < (BN + 31) / 32; ++j) sts(sf + q * C::kSfBytes + 512 + 16 * lane + 4 * j, x[j]);
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::arrive(sf_full(q));
         }
     }
-    T* out = reinterpret_cast<T*>(p.out);
-    for (int i = 0; i < 4; ++i)
-        for (int j = 0; j < 4; ++j) {
-            const int64_t m = m0 + 4 * ty + i, n = n0 + tx + 16 * j;
-            if (m < p.m && n < p.n) out[m * p.ld_out + n] = out_cast<T>(total[i][j] + (p.bias != nullptr ? p.bias[n] : 0.0f));
+    if (warp < 4) {
+        if (!tc::wait(done, 0)) ok = false;
+        __syncwarp();
+        tc::fence_after();
+        // lane = weight row: the sums go to shared memory as (token, 128 rows)
+        float* sums = reinterpret_cast<float*>(smem);
+#pragma unroll
+        for (int c = 0; c < BN; c += 16) {
+            uint32_t v[16];
+            tc::tmem_load16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
+            tc::tmem_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + 32 * warp + lane] = blocks > 0 ? __uint_as_float(v[j]) : 0.0f;
         }
+        tc::fence_before();
+    }
+    if (!ok) atomicOr(&gq_matmul_errors, kErrWaitTimeout);
+    __syncwarp();
+    if (split > 1) tc::cluster_sync();
+    else __syncthreads();
+
+    T* const out = reinterpret_cast<T*>(p.out);
+    const int rows = static_cast<int>(min(static_cast<int64_t>(BN), p.m - m0));
+    for (int u = static_cast<int>(rank) * C::kThreads + tid; u < 32 * rows; u += C::kThreads * split) {
+        const int r = u >> 5, c = 4 * (u & 31);
+        if (n0 + c >= p.n) continue;
+        float v[4] = {0, 0, 0, 0};
+        const uint32_t at = base + (r * 128 + c) * 4;
+        for (int s = 0; s < split; ++s) {
+            const float4 x = split > 1 ? tc::load_cluster(tc::map_shared(at, s)) : *reinterpret_cast<const float4*>(smem + (r * 128 + c) * 4);
+            v[0] = __fadd_rn(v[0], x.x);
+            v[1] = __fadd_rn(v[1], x.y);
+            v[2] = __fadd_rn(v[2], x.z);
+            v[3] = __fadd_rn(v[3], x.w);
+        }
+        if (p.bias != nullptr)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (n0 + c + i < p.n) v[i] = __fadd_rn(v[i], p.bias[n0 + c + i]);
+        store4(out + (m0 + r) * p.ld_out + n0 + c, v, p.n - n0 - c);
+    }
+    // the partial sums stay until every CTA of the cluster has read them
+    if (split > 1) tc::cluster_sync();
+    else __syncthreads();
+    if (warp == 5) {
+        tc::fence_after();
+        tc::tmem_free<C::kCols>(tmem);
+    }
+}
+
+// ---- host side ------------------------------------------------------------------------------
+
+using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeTiled encode_tiled() {
+    static const EncodeTiled fn = [] {
+        void* f = nullptr;
+        cudaDriverEntryPointQueryResult r;
+        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess) f = nullptr;
+        return reinterpret_cast<EncodeTiled>(f);
+    }();
+    return fn;
+}
+
+// (rows, k) bytes with a row stride, in boxes of box_rows x 128 bytes laid out in the
+// 128-byte swizzle
+bool tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {
+    const EncodeTiled fn = encode_tiled();
+    if (fn == nullptr) return false;
+    const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
+    const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
+    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, step,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+int sm_count() {
+    int dev = 0, sms = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    return sms;
+}
+
+template <int BN, class T>
+int launch_narrow(const GqMatmul& p, cudaStream_t s) {
+    using C = Narrow<BN>;
+    auto kern = gq_matmul_narrow<BN, T>;
+    CUtensorMap map_b, map_a;
+    if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, 128) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, BN))
+        return static_cast<int>(cudaErrorInvalidValue);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int64_t tiles = (p.m + BN - 1) / BN * ((p.n + 127) / 128);
+    int split = 1;
+    const int sms = sm_count();
+    while (split < 8 && tiles * split * 2 <= 2 * sms && p.kb >= 4 * split) split *= 2;
+    if (tiles * split > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
+    cfg.blockDim = dim3(C::kThreads);
+    cfg.dynamicSmemBytes = C::kSmem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    e = cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p, split);
+    return static_cast<int>(e);
+}
+
+// out = bias (or 0): a product over no columns
+template <class T>
+__global__ void gq_matmul_bias(const GqMatmul p) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.m * p.n;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t m = i / p.n, n = i - m * p.n;
+        reinterpret_cast<T*>(p.out)[m * p.ld_out + n] = out_cast<T>(p.bias != nullptr ? p.bias[n] : 0.0f);
+    }
 }
 
 template <class T>
 int launch_t(const GqMatmul& p, cudaStream_t s) {
-    const int64_t tiles = (p.m + 63) / 64 * ((p.n + 63) / 64);
-    if (tiles > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
-    gq_matmul_kernel<T><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p);
-    return static_cast<int>(cudaGetLastError());
+    if (p.k == 0) {
+        gq_matmul_bias<T><<<1024, 256, 0, s>>>(p);
+        return static_cast<int>(cudaGetLastError());
+    }
+    if (p.m <= 16) return launch_narrow<16, T>(p, s);
+    if (p.m <= 32) return launch_narrow<32, T>(p, s);
+    if (p.m <= 64) return launch_narrow<64, T>(p, s);
+    return launch_narrow<128, T>(p, s);
 }
 
 }  // namespace
@@ -85,6 +337,17 @@ int launch_matmul(int dtype, const GqMatmul& p, void* stream) {
         case GQ_TYPE_BF16: return launch_t<__nv_bfloat16>(p, s);
         default: return static_cast<int>(cudaErrorInvalidValue);
     }
+}
+
+int matmul_errors(bool clear, uint32_t* flags) {
+    unsigned v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, gq_matmul_errors, sizeof(v));
+    if (e == cudaSuccess && clear && v != 0) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(gq_matmul_errors, &zero, sizeof(zero));
+    }
+    *flags = v;
+    return static_cast<int>(e);
 }
 
 }  // namespace gq

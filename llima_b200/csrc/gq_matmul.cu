@@ -239,6 +239,255 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     }
 }
 
+// ---- wide products ----------------------------------------------------------------------------
+//
+// gq_matmul_wide: a persistent grid of CTA pairs (cta_group::2), each pair on a tile of 256
+// tokens (128 per CTA) x BN output channels; every CTA loads its own tokens' rows and half of
+// the weights' rows, so a pair reads as much from L2 as one CTA with a tile half as wide.
+// Warps 0-7 drain the accumulators into registers, release them and then store; warp 8 loads
+// tiles, warp 9 of the first CTA issues the matrix instructions, warp 10 stages the scales.
+
+template <int BN>
+struct Wide {
+    static constexpr int kThreads = 352;
+    static constexpr int kHalf = BN / 2;                       // weight rows per CTA
+    static constexpr int kStageBytes = 128 * kTileK + kHalf * kTileK;
+    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kSfBytes = 512 + 512 * (BN / 128);
+    static constexpr int kSfCols = 4 + 4 * (BN / 128);
+    static constexpr int kAcc = BN == 256 ? 1 : 2;             // accumulators in tensor memory
+    static constexpr int kBars = 2 * kStages + 2 * kSfSlots + 2 * kAcc;
+    static constexpr int kCols = 512;
+    static constexpr int kSmem = 227 * 1024;                   // all of an SM's, as all of its tensor memory
+    static_assert(1024 + kStages * kStageBytes + kSfSlots * kSfBytes + 8 * kBars + 16 <= kSmem, "shared memory");
+    static_assert(kAcc * BN + kSfSlots * kSfCols <= kCols, "tensor memory");
+};
+
+// 32 bytes to one row of the output: the values of columns n.. (T of 2 or 4 bytes)
+template <class T>
+__device__ __forceinline__ void store_run(T* out, const uint32_t (&w)[8], int64_t left) {
+    constexpr int kPer = 32 / sizeof(T);
+    const uintptr_t a = reinterpret_cast<uintptr_t>(out);
+    if (left >= kPer && (a & 31) == 0) {
+        stg256(out, w);
+    } else if (left >= kPer && (a & 15) == 0) {
+        stg128(out, make_uint4(w[0], w[1], w[2], w[3]));
+        stg128(reinterpret_cast<uint8_t*>(out) + 16, make_uint4(w[4], w[5], w[6], w[7]));
+    } else {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+            if (i < left) {
+                if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(out)[i] = w[i];
+                else reinterpret_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
+            }
+    }
+}
+
+template <class T>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+    T c[2] = {out_cast<T>(x), out_cast<T>(y)};
+    uint32_t w;
+    memcpy(&w, c, sizeof(w));
+    return w;
+}
+
+// Tile t of the order in which pairs take them: bands of 8 row tiles, within a band column by
+// column, so that the tiles in flight share rows of both operands in L2.
+__device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
+    constexpr int kBand = 8;
+    const int band = t / (kBand * tiles_n), in = t - band * (kBand * tiles_n);
+    const int tall = min(kBand, tiles_m - band * kBand);
+    tn = in / tall;
+    tm = band * kBand + in - tn * tall;
+}
+
+template <int BN, class T>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 1)
+    gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
+                   const int tiles_m, const int tiles_n) {
+    using C = Wide<BN>;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
+    const uint32_t sf = base + C::kStages * C::kStageBytes, bars = sf + kSfSlots * C::kSfBytes, slot = bars + 8 * C::kBars;
+    const auto full = [&](int s) { return bars + 8 * s; };
+    const auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
+    const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
+    const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + kSfSlots + s); };
+    const auto acc_full = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + s); };
+    const auto acc_empty = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + C::kAcc + s); };
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const uint32_t rank = tc::cluster_rank();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
+    const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
+
+    if (warp == 9) tc::tmem_alloc_pair<C::kCols>(slot);
+    if (tid == 0) {
+        for (int s = 0; s < C::kStages; ++s) {
+            tc::init(full(s), 2);        // the leader's: both CTAs' loads
+            tc::init(empty(s), 1);
+        }
+        for (int s = 0; s < kSfSlots; ++s) {
+            tc::init(sf_full(s), 2);
+            tc::init(sf_empty(s), 1);
+        }
+        for (int s = 0; s < C::kAcc; ++s) {
+            tc::init(acc_full(s), 1);
+            tc::init(acc_empty(s), 16);  // the leader's: eight warps of both CTAs
+        }
+        mbar_init_fence();
+    }
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    tc::fence_after();
+    const uint32_t tmem = lds_u32(slot);
+
+    bool ok = true;
+    if (warp == 8) {
+        if (lane == 0) {
+            tc::prefetch_map(&map_a);
+            tc::prefetch_map(&map_b);
+            int it = 0;
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                int tm, tn;
+                tile_place(t, tiles_m, tiles_n, tm, tn);
+                const int m0 = tm * 256 + 128 * static_cast<int>(rank), n0 = tn * BN + C::kHalf * static_cast<int>(rank);
+                for (int i = 0; i < blocks; ++i, ++it) {
+                    const int s = it % C::kStages, round = it / C::kStages;
+                    if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+                    const uint32_t bar = tc::map_shared(full(s), 0), at = base + s * C::kStageBytes;
+                    tc::arrive_expect_remote(bar, C::kStageBytes);
+                    tc::load_tile_pair(at, &map_a, i * kTileK, m0, bar);
+                    tc::load_tile_pair(at + 128 * kTileK, &map_b, i * kTileK, n0, bar);
+                }
+            }
+            // the instructions' arrivals on this CTA's barriers, before it may end
+            for (int i = max(0, it - C::kStages); ok && i < it; ++i) ok = tc::wait(empty(i % C::kStages), (i / C::kStages) & 1);
+            // after a wait that gave up, loads may be in flight whose barrier is the other
+            // CTA's: they land long before these 10 ms are over
+            if (!ok)
+                for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
+                }
+        }
+    } else if (warp == 9) {
+        if (lane == 0 && rank == 0) {
+            int it = 0, gi = 0, n = 0;
+            for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+                const int b = n % C::kAcc, use = n / C::kAcc;
+                if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
+                tc::fence_after();
+                for (int i = 0; i < blocks; ++i, ++it) {
+                    const int s = it % C::kStages, q = gi % kSfSlots;
+                    const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
+                    if (i % 4 == 0) {
+                        if (!(ok = tc::wait(sf_full(q), (gi / kSfSlots) & 1))) break;
+                        tc::fence_after();
+                        const uint32_t from = sf + q * C::kSfBytes;
+                        tc::copy_scales_pair(ta, tc::scale_desc(from));
+#pragma unroll
+                        for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
+                    }
+                    if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
+                    tc::fence_after();
+                    const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
+                    const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
+                    const uint32_t idesc = tc::instruction<256, BN>(i % 4);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
+                    tc::commit_pair(empty(s));
+                    if (i % 4 == 3 || i + 1 == blocks) {
+                        tc::commit_pair(sf_empty(q));
+                        ++gi;
+                    }
+                }
+                tc::commit_pair(acc_full(b));
+            }
+        }
+    } else if (warp == 10) {
+        int gi = 0;
+        for (int t = pair; t < tiles && ok; t += pairs) {
+            int tm, tn;
+            tile_place(t, tiles_m, tiles_n, tm, tn);
+            const int64_t m0 = static_cast<int64_t>(tm) * 256 + 128 * rank;
+            const int64_t nb0 = static_cast<int64_t>(tn) * (BN / 128), nbs = (p.n + 127) >> 7;
+            for (int g = 0; g < groups; ++g, ++gi) {
+                const int q = gi % kSfSlots, round = gi / kSfSlots;
+                uint32_t x[4], w[BN / 128];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t m = m0 + 32 * j + lane;
+                    x[j] = m < p.m ? scale_word(p.a_scales + m * p.ld_a_scales, 4 * g, blocks) : 0x7F7F7F7Fu;
+                }
+#pragma unroll
+                for (int j = 0; j < BN / 128; ++j)
+                    w[j] = nb0 + j < nbs ? scale_word(p.b_scales + (nb0 + j) * p.ld_b_scales, 4 * g, blocks) : 0x7F7F7F7Fu;
+                if (round > 0 && !(ok = tc::wait(sf_empty(q), (round - 1) & 1))) break;
+                const uint32_t to = sf + q * C::kSfBytes + 16 * lane;
+                sts(to, make_uint4(x[0], x[1], x[2], x[3]));
+#pragma unroll
+                for (int j = 0; j < BN / 128; ++j) sts(to + 512 + 512 * j, make_uint4(w[j], w[j], w[j], w[j]));
+                tc::fence_async_shared();
+                __syncwarp();
+                if (lane == 0) tc::arrive_remote(tc::map_shared(sf_full(q), 0));
+            }
+        }
+        for (int i = max(0, gi - kSfSlots); ok && i < gi; ++i) ok = tc::wait(sf_empty(i % kSfSlots), (i / kSfSlots) & 1);
+    } else {
+        constexpr int kPart = BN / 2;                       // columns per warp
+        constexpr int kWords = sizeof(T) == 4 ? kPart : kPart / 2;
+        int n = 0;
+        for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+            int tm, tn;
+            tile_place(t, tiles_m, tiles_n, tm, tn);
+            const int b = n % C::kAcc, use = n / C::kAcc;
+            if (!(ok = tc::wait(acc_full(b), use & 1))) break;
+            __syncwarp();
+            tc::fence_after();
+            const int64_t m = static_cast<int64_t>(tm) * 256 + 128 * rank + 32 * (warp & 3) + lane;
+            const int64_t n0 = static_cast<int64_t>(tn) * BN + kPart * (warp >> 2);
+            const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + BN * b + kPart * (warp >> 2);
+            uint32_t w[kWords];
+#pragma unroll
+            for (int c = 0; c < kPart; c += 32) {
+                uint32_t v[32];
+                tc::tmem_load32(from + c, v);
+                tc::tmem_wait();
+                if (p.bias != nullptr) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (n0 + c + i < p.n) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), __ldg(p.bias + n0 + c + i)));
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    if constexpr (sizeof(T) == 4) w[c + i] = v[i];
+                    else if (i % 2 == 0) w[(c + i) / 2] = pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                }
+            }
+            tc::fence_before();
+            __syncwarp();
+            if (lane == 0) tc::arrive_remote(tc::map_shared(acc_empty(b), 0));
+            if (m < p.m) {
+                T* const out = reinterpret_cast<T*>(p.out) + m * p.ld_out + n0;
+                constexpr int kPer = 32 / sizeof(T);
+#pragma unroll
+                for (int c = 0; c < kWords; c += 8) {
+                    const uint32_t run[8] = {w[c], w[c + 1], w[c + 2], w[c + 3], w[c + 4], w[c + 5], w[c + 6], w[c + 7]};
+                    store_run<T>(out + c / 8 * kPer, run, p.n - n0 - c / 8 * kPer);
+                }
+            }
+        }
+    }
+    if (!ok) atomicOr(&gq_matmul_errors, kErrWaitTimeout);
+    __syncwarp();
+    tc::fence_before();
+    __syncthreads();
+    tc::cluster_sync();
+    if (warp == 9) {
+        tc::fence_after();
+        tc::tmem_free_pair<C::kCols>(tmem);
+    }
+}
+
 // ---- host side ------------------------------------------------------------------------------
 
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -305,6 +554,23 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     return static_cast<int>(e);
 }
 
+template <int BN, class T>
+int launch_wide(const GqMatmul& p, cudaStream_t s) {
+    using C = Wide<BN>;
+    auto kern = gq_matmul_wide<BN, T>;
+    CUtensorMap map_b, map_a;
+    if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
+        return static_cast<int>(cudaErrorInvalidValue);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    if (e != cudaSuccess) return static_cast<int>(e);
+    const int64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + BN - 1) / BN;
+    if (tiles_m * tiles_n * p.kb > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
+    const int64_t pairs = sm_count() / 2;
+    const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
+    kern<<<grid, C::kThreads, C::kSmem, s>>>(map_a, map_b, p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
+    return static_cast<int>(cudaGetLastError());
+}
+
 // out = bias (or 0): a product over no columns
 template <class T>
 __global__ void gq_matmul_bias(const GqMatmul p) {
@@ -324,7 +590,10 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.m <= 16) return launch_narrow<16, T>(p, s);
     if (p.m <= 32) return launch_narrow<32, T>(p, s);
     if (p.m <= 64) return launch_narrow<64, T>(p, s);
-    return launch_narrow<128, T>(p, s);
+    if (p.m <= 256) return launch_narrow<128, T>(p, s);
+    const int64_t wide = (p.m + 255) / 256 * ((p.n + 255) / 256);
+    if (2 * wide >= sm_count()) return launch_wide<256, T>(p, s);
+    return launch_wide<128, T>(p, s);
 }
 
 }  // namespace

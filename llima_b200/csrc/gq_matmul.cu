@@ -99,7 +99,8 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
     const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + kSfSlots + s); };
     const uint32_t done = bars + 8 * (C::kBars - 1);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform for the compiler
 
     const uint32_t rank = split > 1 ? tc::cluster_rank() : 0;
     const int64_t tile = blockIdx.x / split;
@@ -128,36 +129,40 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
 
     bool ok = true;
     if (warp == 4) {
-        if (lane == 0) {
+        if (tc::elect()) {
             tc::prefetch_map(&map_b);
             tc::prefetch_map(&map_a);
-            int issued = 0;
-            for (int i = 0; i < blocks; ++i) {
-                const int s = i % C::kStages, round = i / C::kStages;
-                if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+        }
+        int issued = 0;
+        for (int i = 0; i < blocks; ++i) {
+            const int s = i % C::kStages, round = i / C::kStages;
+            if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+            if (tc::elect()) {
                 tc::arrive_expect(full(s), C::kStageBytes);
                 const uint32_t at = base + s * C::kStageBytes;
                 tc::load_tile(at, &map_b, (kb0 + i) * kTileK, static_cast<int>(n0), full(s));
                 tc::load_tile(at + 128 * kTileK, &map_a, (kb0 + i) * kTileK, static_cast<int>(m0), full(s));
-                issued = i + 1;
             }
-            // nothing of this CTA is in flight when it ends, also after a wait that gave up
-            if (!ok)
-                for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
+            issued = i + 1;
         }
+        // nothing of this CTA is in flight when it ends, also after a wait that gave up
+        if (!ok)
+            for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
     } else if (warp == 5) {
-        if (lane == 0) {
-            for (int i = 0; i < blocks; ++i) {
-                const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
-                const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
-                if (i % 4 == 0) {
-                    if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
-                    tc::fence_after();
+        for (int i = 0; i < blocks; ++i) {
+            const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
+            const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
+            if (i % 4 == 0) {
+                if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
+                tc::fence_after();
+                if (tc::elect()) {
                     tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
                     tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
                 }
-                if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
-                tc::fence_after();
+            }
+            if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
+            tc::fence_after();
+            if (tc::elect()) {
                 const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
                 const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
                 const uint32_t idesc = tc::instruction<128, BN>(i % 4);
@@ -166,8 +171,9 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
                 tc::commit(empty(s));
                 if (i % 4 == 3 || i + 1 == blocks) tc::commit(sf_empty(q));
             }
-            tc::commit(done);
+            __syncwarp();
         }
+        if (tc::elect()) tc::commit(done);
     } else if (warp == 2) {
         // scales: the weights' byte is the same for all 128 rows of the tile
         const uint8_t* wrow = p.b_scales + (n0 >> 7) * p.ld_b_scales;
@@ -315,7 +321,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
     const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + kSfSlots + s); };
     const auto acc_full = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + s); };
     const auto acc_empty = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + C::kAcc + s); };
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform for the compiler
     const uint32_t rank = tc::cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
     const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
@@ -323,7 +330,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
     if (warp == 9) tc::tmem_alloc_pair<C::kCols>(slot);
     if (tid == 0) {
         for (int s = 0; s < C::kStages; ++s) {
-            tc::init(full(s), 2);        // the leader's: both CTAs' loads
+            tc::init(full(s), 1);        // the first CTA's: both CTAs' loads
             tc::init(empty(s), 1);
         }
         for (int s = 0; s < kSfSlots; ++s) {
@@ -332,7 +339,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
         }
         for (int s = 0; s < C::kAcc; ++s) {
             tc::init(acc_full(s), 1);
-            tc::init(acc_empty(s), 16);  // the leader's: eight warps of both CTAs
+            tc::init(acc_empty(s), 16);  // the first CTA's: eight warps of both CTAs
         }
         mbar_init_fence();
     }
@@ -344,64 +351,71 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
 
     bool ok = true;
     if (warp == 8) {
-        if (lane == 0) {
+        if (tc::elect()) {
             tc::prefetch_map(&map_a);
             tc::prefetch_map(&map_b);
-            int it = 0;
-            for (int t = pair; t < tiles && ok; t += pairs) {
-                int tm, tn;
-                tile_place(t, tiles_m, tiles_n, tm, tn);
-                const int m0 = tm * 256 + 128 * static_cast<int>(rank), n0 = tn * BN + C::kHalf * static_cast<int>(rank);
-                for (int i = 0; i < blocks; ++i, ++it) {
-                    const int s = it % C::kStages, round = it / C::kStages;
-                    if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+        }
+        int it = 0;
+        for (int t = pair; t < tiles && ok; t += pairs) {
+            int tm, tn;
+            tile_place(t, tiles_m, tiles_n, tm, tn);
+            const int m0 = tm * 256 + 128 * static_cast<int>(rank), n0 = tn * BN + C::kHalf * static_cast<int>(rank);
+            for (int i = 0; i < blocks; ++i, ++it) {
+                const int s = it % C::kStages, round = it / C::kStages;
+                if (round > 0 && !(ok = tc::wait(empty(s), (round - 1) & 1))) break;
+                if (tc::elect()) {
                     const uint32_t bar = tc::map_shared(full(s), 0), at = base + s * C::kStageBytes;
-                    tc::arrive_expect_remote(bar, C::kStageBytes);
+                    // the first CTA expects both CTAs' bytes; the second's may land before: its
+                    // loads wait for the instructions that used the stage, so for this phase
+                    if (rank == 0) tc::arrive_expect(full(s), 2 * C::kStageBytes);
                     tc::load_tile_pair(at, &map_a, i * kTileK, m0, bar);
                     tc::load_tile_pair(at + 128 * kTileK, &map_b, i * kTileK, n0, bar);
                 }
             }
-            // the instructions' arrivals on this CTA's barriers, before it may end
-            for (int i = max(0, it - C::kStages); ok && i < it; ++i) ok = tc::wait(empty(i % C::kStages), (i / C::kStages) & 1);
-            // after a wait that gave up, loads may be in flight whose barrier is the other
-            // CTA's: they land long before these 10 ms are over
-            if (!ok)
-                for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
-                }
         }
+        // the instructions' arrivals on this CTA's barriers, before it may end
+        for (int i = max(0, it - C::kStages); ok && i < it; ++i) ok = tc::wait(empty(i % C::kStages), (i / C::kStages) & 1);
+        // after a wait that gave up, loads may be in flight whose barrier is the other CTA's:
+        // they land long before these 10 ms are over
+        if (!ok)
+            for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
+            }
     } else if (warp == 9) {
-        if (lane == 0 && rank == 0) {
-            int it = 0, gi = 0, n = 0;
-            for (int t = pair; t < tiles && ok; t += pairs, ++n) {
-                const int b = n % C::kAcc, use = n / C::kAcc;
-                if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
-                tc::fence_after();
-                for (int i = 0; i < blocks; ++i, ++it) {
-                    const int s = it % C::kStages, q = gi % kSfSlots;
-                    const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
-                    if (i % 4 == 0) {
-                        if (!(ok = tc::wait(sf_full(q), (gi / kSfSlots) & 1))) break;
-                        tc::fence_after();
+        int it = 0, gi = 0, n = 0;
+        for (int t = pair; rank == 0 && t < tiles && ok; t += pairs, ++n) {
+            const int b = n % C::kAcc, use = n / C::kAcc;
+            if (use > 0 && !(ok = tc::wait<true>(acc_empty(b), (use - 1) & 1))) break;
+            tc::fence_after();
+            for (int i = 0; i < blocks; ++i, ++it) {
+                const int s = it % C::kStages, q = gi % kSfSlots;
+                const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
+                if (i % 4 == 0) {
+                    if (!(ok = tc::wait<true>(sf_full(q), (gi / kSfSlots) & 1))) break;
+                    tc::fence_after();
+                    if (tc::elect()) {
                         const uint32_t from = sf + q * C::kSfBytes;
                         tc::copy_scales_pair(ta, tc::scale_desc(from));
 #pragma unroll
                         for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
                     }
-                    if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
-                    tc::fence_after();
+                }
+                if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
+                tc::fence_after();
+                const bool last = i % 4 == 3 || i + 1 == blocks;
+                if (tc::elect()) {
                     const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
                     const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
                     const uint32_t idesc = tc::instruction<256, BN>(i % 4);
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
                     tc::commit_pair(empty(s));
-                    if (i % 4 == 3 || i + 1 == blocks) {
-                        tc::commit_pair(sf_empty(q));
-                        ++gi;
-                    }
+                    if (last) tc::commit_pair(sf_empty(q));
                 }
-                tc::commit_pair(acc_full(b));
+                __syncwarp();
+                if (last) ++gi;
             }
+            if (tc::elect()) tc::commit_pair(acc_full(b));
+            __syncwarp();
         }
     } else if (warp == 10) {
         int gi = 0;

@@ -384,13 +384,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
         int it = 0, gi = 0, n = 0;
         for (int t = pair; rank == 0 && t < tiles && ok; t += pairs, ++n) {
             const int b = n % C::kAcc, use = n / C::kAcc;
-            if (use > 0 && !(ok = tc::wait<true>(acc_empty(b), (use - 1) & 1))) break;
+            if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
             tc::fence_after();
             for (int i = 0; i < blocks; ++i, ++it) {
                 const int s = it % C::kStages, q = gi % kSfSlots;
                 const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
                 if (i % 4 == 0) {
-                    if (!(ok = tc::wait<true>(sf_full(q), (gi / kSfSlots) & 1))) break;
+                    if (!(ok = tc::wait(sf_full(q), (gi / kSfSlots) & 1))) break;
                     tc::fence_after();
                     if (tc::elect()) {
                         const uint32_t from = sf + q * C::kSfBytes;
@@ -448,7 +448,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
         for (int i = max(0, gi - kSfSlots); ok && i < gi; ++i) ok = tc::wait(sf_empty(i % kSfSlots), (i / kSfSlots) & 1);
     } else {
         constexpr int kPart = BN / 2;                       // columns per warp
-        constexpr int kWords = sizeof(T) == 4 ? kPart : kPart / 2;
         int n = 0;
         for (int t = pair; t < tiles && ok; t += pairs, ++n) {
             int tm, tn;
@@ -460,33 +459,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
             const int64_t m = static_cast<int64_t>(tm) * 256 + 128 * rank + 32 * (warp & 3) + lane;
             const int64_t n0 = static_cast<int64_t>(tn) * BN + kPart * (warp >> 2);
             const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + BN * b + kPart * (warp >> 2);
-            uint32_t w[kWords];
+            // the accumulators are free for the next tile once they are in registers
+            uint32_t v[kPart];
 #pragma unroll
-            for (int c = 0; c < kPart; c += 32) {
-                uint32_t v[32];
-                tc::tmem_load32(from + c, v);
-                tc::tmem_wait();
-                if (p.bias != nullptr) {
-#pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (n0 + c + i < p.n) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), __ldg(p.bias + n0 + c + i)));
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    if constexpr (sizeof(T) == 4) w[c + i] = v[i];
-                    else if (i % 2 == 0) w[(c + i) / 2] = pack2<T>(__uint_as_float(v[i]), __uint_as_float(v[i + 1]));
-                }
-            }
+            for (int c = 0; c < kPart; c += 32) tc::tmem_load32(from + c, v + c);
+            tc::tmem_wait();
             tc::fence_before();
             __syncwarp();
             if (lane == 0) tc::arrive_remote(tc::map_shared(acc_empty(b), 0));
+            if (p.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < kPart; ++i)
+                    if (n0 + i < p.n) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), __ldg(p.bias + n0 + i)));
+            }
             if (m < p.m) {
                 T* const out = reinterpret_cast<T*>(p.out) + m * p.ld_out + n0;
                 constexpr int kPer = 32 / sizeof(T);
 #pragma unroll
-                for (int c = 0; c < kWords; c += 8) {
-                    const uint32_t run[8] = {w[c], w[c + 1], w[c + 2], w[c + 3], w[c + 4], w[c + 5], w[c + 6], w[c + 7]};
-                    store_run<T>(out + c / 8 * kPer, run, p.n - n0 - c / 8 * kPer);
+                for (int c = 0; c < kPart; c += kPer) {
+                    uint32_t run[8];
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if constexpr (sizeof(T) == 4) run[i] = v[c + i];
+                        else run[i] = pack2<T>(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1]));
+                    }
+                    store_run<T>(out + c, run, p.n - n0 - c);
                 }
             }
         }

@@ -14,7 +14,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <mutex>
+#include <atomic>
 
 #include "gq_internal.h"
 #include "gq_tcgen05.cuh"
@@ -535,6 +535,19 @@ int sm_count() {
     return sms;
 }
 
+// The kernel's shared memory limit, raised once per device and kernel (`done`: a bit per device).
+template <class K>
+cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    const cudaError_t g = cudaGetDevice(&dev);
+    if (g != cudaSuccess) return g;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
+    return e;
+}
+
 template <int BN, class T>
 int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     using C = Narrow<BN>;
@@ -542,7 +555,8 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     CUtensorMap map_b, map_a;
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, 128) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, BN))
         return static_cast<int>(cudaErrorInvalidValue);
-    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles = (p.m + BN - 1) / BN * ((p.n + 127) / 128);
     int split = 1;
@@ -572,7 +586,8 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
     CUtensorMap map_b, map_a;
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
         return static_cast<int>(cudaErrorInvalidValue);
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + BN - 1) / BN;
     if (tiles_m * tiles_n * p.kb > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);

@@ -37,6 +37,8 @@ __all__ = ["Fp8Rows", "Fp8Weight", "convert_fp8_device", "fp8_from_gguf", "rms_n
 
 BLOCK = 128
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
 _TYPE_IDS = {torch.float32: FORMATS["F32"].type_id, torch.float16: FORMATS["F16"].type_id,
              torch.bfloat16: FORMATS["BF16"].type_id}
 
@@ -55,34 +57,26 @@ class Fp8Weight(NamedTuple):
     scales: torch.Tensor
 
 
-class _On:
-    """The device of a call made current, and its current stream."""
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, device: torch.device):
-        self.guard = None
-        if device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+def _call(name: str, device: int, *args) -> None:
+    """The C entry point `name` with the current stream of CUDA device `device`, which is made
+    current for the call.  (``torch.cuda.current_stream`` builds a Stream object, 3 us a call;
+    its handle alone is what the C ABI takes.)"""
+    if device == _current_device():
+        status = getattr(N.lib(), name)(*args, _raw_stream(device))
+    else:
+        with torch.cuda.device(device):
+            status = getattr(N.lib(), name)(*args, _raw_stream(device))
+    if status:
+        N.check(status, name)
 
 
-def _matrix(t: torch.Tensor, name: str, dtype, device: torch.device | None, rows: int | None = None,
-            cols: int | None = None) -> int:
-    """Checks a 2-D CUDA operand whose rows are consecutive elements; returns its row stride."""
+def _matrix(t: torch.Tensor, name: str, dtype, device: int, rows: int | None = None, cols: int | None = None) -> int:
+    """Checks a 2-D operand on CUDA device `device` whose rows are consecutive elements;
+    returns its row stride."""
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
-    if not t.is_cuda:
-        raise TypeError(f"{name} must be a CUDA tensor")
-    if device is not None and t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+    if t.get_device() != device:
+        raise ValueError(f"{name} is on {t.device}, the other operands on cuda:{device}")
     if t.dim() != 2:
         raise ValueError(f"{name} must have two dimensions, not {t.dim()}")
     r, c = t.shape
@@ -90,7 +84,7 @@ def _matrix(t: torch.Tensor, name: str, dtype, device: torch.device | None, rows
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected "
                          f"{(r if rows is None else rows, c if cols is None else cols)}")
     s0, s1 = t.stride()
-    if c > 1 and s1 != 1:
+    if s1 != 1 and c > 1:
         raise ValueError(f"the elements of a row of {name} must be consecutive (strides {t.stride()})")
     if r <= 1:
         return c
@@ -99,21 +93,38 @@ def _matrix(t: torch.Tensor, name: str, dtype, device: torch.device | None, rows
     return s0
 
 
+def _device_of(t: torch.Tensor, name: str) -> int:
+    if not t.is_cuda:
+        raise TypeError(f"{name} must be a CUDA tensor")
+    return t.get_device()
+
+
+def _vector(t: torch.Tensor, name: str, n: int, device: int) -> int:
+    """Checks `n` consecutive float32 values on CUDA device `device`; returns their address."""
+    if t.dtype is not torch.float32 or t.shape != (n,) or t.get_device() != device or (t.stride(0) != 1 and n > 1):
+        raise ValueError(f"{name} must be a contiguous float32 tensor of {n} values on cuda:{device}")
+    return t.data_ptr()
+
+
 def _float_rows(x: torch.Tensor, name: str) -> int:
     if x.dtype not in _TYPE_IDS:
         raise TypeError(f"{name} must be float32, float16 or bfloat16, not {x.dtype}")
-    if x.dim() == 2 and x.shape[1] % 32:
+    ld = _matrix(x, name, x.dtype, _device_of(x, name))
+    if x.shape[1] % 32:
         raise ValueError(f"{name} has {x.shape[1]} columns: a multiple of 32 is needed")
-    return _matrix(x, name, x.dtype, None)
+    return ld
 
 
-def _rows_out(rows: int, cols: int, device, out: Fp8Rows | None):
-    blocks = (cols + BLOCK - 1) // BLOCK
+def _rows_out(x: torch.Tensor, device: int, out: Fp8Rows | None):
+    """The codes and scales that rows shaped like x go to, with their row strides."""
+    rows, cols = x.shape
+    blocks = (cols + 127) >> 7
     if out is None:
-        return Fp8Rows(torch.empty((rows, cols), dtype=E4M3, device=device),
-                       torch.empty((rows, blocks), dtype=E8M0, device=device)), cols, blocks
-    ld = _matrix(out.codes, "out.codes", E4M3, device, rows, cols)
-    return out, ld, _matrix(out.scales, "out.scales", E8M0, device, rows, blocks)
+        return (torch.empty_like(x, dtype=E4M3, memory_format=torch.contiguous_format), cols,
+                x.new_empty((rows, blocks), dtype=E8M0), blocks)
+    codes, scales = out
+    return (codes, _matrix(codes, "out.codes", E4M3, device, rows, cols),
+            scales, _matrix(scales, "out.scales", E8M0, device, rows, blocks))
 
 
 def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads: int = 0,
@@ -124,21 +135,20 @@ def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads:
     f = FORMATS[fmt]
     if src.dtype != torch.uint8 or not src.is_cuda or not src.is_contiguous():
         raise TypeError("src must be a contiguous CUDA uint8 tensor of GGUF bytes")
+    dev = src.get_device()
     shape = ((rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
     if out is None:
         if rows < 0 or cols < 0:
             raise ValueError(f"negative shape ({rows}, {cols})")
-        out = Fp8Weight(torch.empty((rows, cols), dtype=E4M3, device=src.device),
-                        torch.empty(shape, dtype=E8M0, device=src.device))
+        out = Fp8Weight(src.new_empty((rows, cols), dtype=E4M3), src.new_empty(shape, dtype=E8M0))
     else:
-        _matrix(out.codes, "out.codes", E4M3, src.device, rows, cols)
-        _matrix(out.scales, "out.scales", E8M0, src.device, *shape)
+        _matrix(out.codes, "out.codes", E4M3, dev, rows, cols)
+        _matrix(out.scales, "out.scales", E8M0, dev, *shape)
         if not out.codes.is_contiguous() or not out.scales.is_contiguous():
             raise ValueError("out must be contiguous")
     t = N.Tensor(type=f.type_id, perm_heads=heads, rows=rows, cols=cols, src=src.data_ptr(), src_bytes=src.numel(),
                  codes=out.codes.data_ptr())
-    with _On(src.device) as stream:
-        N.check(N.lib().gq_convert_fp8(ctypes.byref(t), out.scales.data_ptr(), stream), "gq_convert_fp8")
+    _call("gq_convert_fp8", dev, ctypes.byref(t), out.scales.data_ptr())
     return out
 
 
@@ -165,25 +175,24 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
     ``sum_out`` receives h and may be ``residual`` or ``x`` itself."""
     ld_x = _float_rows(x, "x")
     rows, cols = x.shape
-    dev = x.device
-    if weight.dtype != torch.float32 or weight.shape != (cols,) or weight.device != dev or not weight.is_contiguous():
-        raise ValueError(f"weight must be a contiguous float32 tensor of {cols} values on {dev}")
+    dev = x.get_device()
+    w = _vector(weight, "weight", cols, dev)
     ld_r = ld_s = 0
+    r = s = None
     if residual is not None:
         ld_r = _matrix(residual, "residual", x.dtype, dev, rows, cols)
         if sum_out is None:
-            sum_out = torch.empty((rows, cols), dtype=x.dtype, device=dev)
-        ld_s = _matrix(sum_out, "sum_out", x.dtype, dev, rows, cols)
+            sum_out, ld_s = torch.empty_like(x, memory_format=torch.contiguous_format), cols
+        else:
+            ld_s = _matrix(sum_out, "sum_out", x.dtype, dev, rows, cols)
+        r, s = residual.data_ptr(), sum_out.data_ptr()
     elif sum_out is not None:
         raise ValueError("sum_out without residual")
-    out, ld_c, ld_sc = _rows_out(rows, cols, dev, out)
-    with _On(dev) as stream:
-        N.check(N.lib().gq_rms_norm_fp8(_TYPE_IDS[x.dtype], x.data_ptr(), ld_x,
-                                        None if residual is None else residual.data_ptr(), ld_r, weight.data_ptr(), eps,
-                                        rows, cols, None if residual is None else sum_out.data_ptr(), ld_s,
-                                        out.codes.data_ptr(), ld_c, out.scales.data_ptr(), ld_sc, stream),
-                "gq_rms_norm_fp8")
-    return out if residual is None else (out, sum_out)
+    codes, ld_c, scales, ld_sc = _rows_out(x, dev, out)
+    _call("gq_rms_norm_fp8", dev, _TYPE_IDS[x.dtype], x.data_ptr(), ld_x, r, ld_r, w, eps, rows, cols, s, ld_s,
+          codes.data_ptr(), ld_c, scales.data_ptr(), ld_sc)
+    q = Fp8Rows(codes, scales)
+    return q if residual is None else (q, sum_out)
 
 
 def quantize_fp8(x: torch.Tensor, gate: torch.Tensor | None = None, out: Fp8Rows | None = None) -> Fp8Rows:
@@ -192,13 +201,14 @@ def quantize_fp8(x: torch.Tensor, gate: torch.Tensor | None = None, out: Fp8Rows
     product leaves them."""
     ld_x = _float_rows(x, "x")
     rows, cols = x.shape
-    ld_g = 0 if gate is None else _matrix(gate, "gate", x.dtype, x.device, rows, cols)
-    out, ld_c, ld_sc = _rows_out(rows, cols, x.device, out)
-    with _On(x.device) as stream:
-        N.check(N.lib().gq_quantize_fp8(_TYPE_IDS[x.dtype], x.data_ptr(), ld_x, None if gate is None else gate.data_ptr(),
-                                        ld_g, rows, cols, out.codes.data_ptr(), ld_c, out.scales.data_ptr(), ld_sc,
-                                        stream), "gq_quantize_fp8")
-    return out
+    dev = x.get_device()
+    ld_g, g = 0, None
+    if gate is not None:
+        ld_g, g = _matrix(gate, "gate", x.dtype, dev, rows, cols), gate.data_ptr()
+    codes, ld_c, scales, ld_sc = _rows_out(x, dev, out)
+    _call("gq_quantize_fp8", dev, _TYPE_IDS[x.dtype], x.data_ptr(), ld_x, g, ld_g, rows, cols, codes.data_ptr(), ld_c,
+          scales.data_ptr(), ld_sc)
+    return Fp8Rows(codes, scales)
 
 
 def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
@@ -208,32 +218,28 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     rounded once.  ``out`` must not overlap the operands."""
     codes, scales = a
     w_codes, w_scales = w
-    dev = codes.device
-    ld_a = _matrix(codes, "a.codes", E4M3, None)
+    dev = _device_of(codes, "a.codes")
+    ld_a = _matrix(codes, "a.codes", E4M3, dev)
     m, k = codes.shape
     if k % 32:
         raise ValueError(f"a.codes has {k} columns: a multiple of 32 is needed")
-    blocks = (k + BLOCK - 1) // BLOCK
+    blocks = (k + 127) >> 7
     ld_sa = _matrix(scales, "a.scales", E8M0, dev, m, blocks)
     ld_b = _matrix(w_codes, "w.codes", E4M3, dev, None, k)
     n = w_codes.shape[0]
-    ld_sb = _matrix(w_scales, "w.scales", E8M0, dev, (n + BLOCK - 1) // BLOCK, blocks)
-    if bias is not None and (bias.dtype != torch.float32 or bias.shape != (n,) or bias.device != dev
-                             or not bias.is_contiguous()):
-        raise ValueError(f"bias must be a contiguous float32 tensor of {n} values on {dev}")
+    ld_sb = _matrix(w_scales, "w.scales", E8M0, dev, (n + 127) >> 7, blocks)
     if out is None:
         if dtype not in _TYPE_IDS:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
-        out = torch.empty((m, n), dtype=dtype, device=dev)
-        ld_o = n
+        out, ld_o = codes.new_empty((m, n), dtype=dtype), n
     else:
-        if out.dtype not in _TYPE_IDS:
-            raise TypeError(f"out must be float32, float16 or bfloat16, not {out.dtype}")
-        ld_o = _matrix(out, "out", out.dtype, dev, m, n)
-    with _On(dev) as stream:
-        N.check(N.lib().gq_matmul_fp8(codes.data_ptr(), ld_a, scales.data_ptr(), ld_sa, w_codes.data_ptr(), ld_b,
-                                      w_scales.data_ptr(), ld_sb, None if bias is None else bias.data_ptr(), m, n, k,
-                                      _TYPE_IDS[out.dtype], out.data_ptr(), ld_o, stream), "gq_matmul_fp8")
+        dtype = out.dtype
+        if dtype not in _TYPE_IDS:
+            raise TypeError(f"out must be float32, float16 or bfloat16, not {dtype}")
+        ld_o = _matrix(out, "out", dtype, dev, m, n)
+    _call("gq_matmul_fp8", dev, codes.data_ptr(), ld_a, scales.data_ptr(), ld_sa, w_codes.data_ptr(), ld_b,
+          w_scales.data_ptr(), ld_sb, None if bias is None else _vector(bias, "bias", n, dev), m, n, k, _TYPE_IDS[dtype],
+          out.data_ptr(), ld_o)
     return out
 
 

@@ -253,8 +253,8 @@ GQ_API int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stre
  * residual is NULL), y = h / sqrt(mean(h^2) + eps) * weight in f32, y as e4m3 codes
  * (rows, cols) with one scale per 1 x 128 block (rows, ceil(cols/128)).  dtype (of x,
  * residual and sum): GQ_TYPE_F32, F16 or BF16; weight: f32 (cols).  sum receives h when
- * residual is given and may be residual or x itself.  cols a multiple of 32; rows at most
- * 2^31 - 1; every row of x, residual, sum and codes starts on a 16-byte boundary, and weight
+ * residual is given and may be residual or x itself.  cols a multiple of 32; rows and
+ * cols at most 2^31 - 1; every row of x, residual, sum and codes starts on a 16-byte boundary, and weight
  * does. */
 GQ_API int gq_rms_norm_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* residual, int64_t ld_residual,
                            const float* weight, float eps, int64_t rows, int64_t cols, void* sum, int64_t ld_sum,

@@ -141,7 +141,7 @@ constexpr int64_t kMaxStride = int64_t(1) << 38;   // the limit of a tensor map'
 
 int rows_check(int64_t rows, int64_t cols) {
     if (rows < 0 || cols < 0 || cols % 32 != 0) return GQ_ERR_SIZE;
-    if (rows > INT32_MAX || (cols != 0 && rows > INT64_MAX / 4 / cols)) return GQ_ERR_SIZE;
+    if (rows > INT32_MAX || cols > INT32_MAX) return GQ_ERR_SIZE;
     return GQ_OK;
 }
 

@@ -39,7 +39,15 @@ struct BlockView {
                                                              : 210;
 };
 
-template <int TYPE>
+// 16 bytes of a unit: rows of 16-byte units at 16-byte addresses (UNITS16) in one load
+template <bool UNITS16>
+__device__ __forceinline__ uint4 unit_bytes16(const uint8_t* p) {
+    if constexpr (UNITS16) return lds128(p);
+    else return lds128_align2(p);
+}
+
+// UNITS16: the row starts at a 16-byte address (which Q4_K's and Q5_K's units then do as well)
+template <int TYPE, bool UNITS16 = false>
 __device__ __forceinline__ void decode_block(const uint8_t* row, int b, uint32_t (&w)[8], float& A, float& B) {
     B = 0.0f;
     if constexpr (TYPE == GQ_TYPE_Q6_K) {
@@ -69,12 +77,12 @@ __device__ __forceinline__ void decode_block(const uint8_t* row, int b, uint32_t
         A = __fmul_rn(h2f(lds16(sp)), static_cast<float>(sc));
         B = __fmul_rn(h2f(lds16(sp + 2)), static_cast<float>(mn));
         const uint8_t* qp = sp + (Q5 ? 48 : 16) + 32 * g;
-        const uint4 a0 = lds128_align2(qp), a1 = lds128_align2(qp + 16);
+        const uint4 a0 = unit_bytes16<UNITS16>(qp), a1 = unit_bytes16<UNITS16>(qp + 16);
         const uint32_t x[8] = {a0.x, a0.y, a0.z, a0.w, a1.x, a1.y, a1.z, a1.w};
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] = (x[i] >> (4 * (k & 1))) & 0x0F0F0F0Fu;
         if constexpr (Q5) {
-            const uint4 c0 = lds128_align2(sp + 16), c1 = lds128_align2(sp + 32);
+            const uint4 c0 = unit_bytes16<UNITS16>(sp + 16), c1 = unit_bytes16<UNITS16>(sp + 32);
             const uint32_t hb[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) w[i] |= ((hb[i] >> k) & 0x01010101u) << 4;

@@ -228,12 +228,13 @@ int gq_kernel_errors(int32_t device, int32_t clear, uint32_t* flags) {
     *flags = 0;
     const DeviceScope scope(device);
     if (scope.status() != GQ_OK) return scope.status();
-    uint32_t more = 0;
-    const int st = cuda_status(gq::kernel_errors(clear != 0, flags));
-    if (st != GQ_OK) return st;
-    const int sm = cuda_status(gq::matmul_errors(clear != 0, &more));
-    *flags |= more;
-    return sm;
+    for (int (*read)(bool, uint32_t*) : {gq::kernel_errors, gq::fp8_errors, gq::matmul_errors}) {
+        uint32_t f = 0;
+        const int st = cuda_status(read(clear != 0, &f));
+        if (st != GQ_OK) return st;
+        *flags |= f;
+    }
+    return GQ_OK;
 }
 
 int gq_query(int32_t type, int64_t rows, int64_t cols, gq_layout_t* out) {
@@ -517,7 +518,7 @@ int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream) {
     int64_t nv = 0, nu = 0;
     const int st = shape_check(t, &ti, &nv, &nu);
     if (st != GQ_OK) return st;
-    if (t.cols % 32 != 0) return GQ_ERR_SIZE;
+    if (t.cols % 32 != 0 || t.rows > INT32_MAX) return GQ_ERR_SIZE;
     if (nv == 0) return GQ_OK;
     if (t.src == nullptr || t.codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
     if (!aligned(t.src, 16) || !aligned(t.codes, 16)) return GQ_ERR_ALIGN;
@@ -531,10 +532,7 @@ int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream) {
     p.src_bytes = nu * ti.unit_bytes;
     p.scale_cols = (t.cols + 127) / 128;
     if ((t.rows + 127) / 128 > INT32_MAX / p.scale_cols) return GQ_ERR_SIZE;
-    if (t.perm_heads > 0) {
-        if (t.rows / t.perm_heads > INT32_MAX) return GQ_ERR_SIZE;
-        p.head_dim = static_cast<int32_t>(t.rows / t.perm_heads);
-    }
+    if (t.perm_heads > 0) p.head_dim = static_cast<uint32_t>(t.rows / t.perm_heads);
     return cuda_status(gq::launch_fp8_weight(t.type, p, stream));
 }
 

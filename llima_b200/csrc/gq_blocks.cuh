@@ -46,6 +46,20 @@ __device__ __forceinline__ uint4 unit_bytes16(const uint8_t* p) {
     else return lds128_align2(p);
 }
 
+// 32 bytes at a 2-byte-aligned shared address as eight words
+__device__ __forceinline__ void load32_align2(const uint8_t* p, uint32_t (&x)[8]) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
+    const uint32_t sh = static_cast<uint32_t>(a & 3u) * 8u;
+    uint32_t prev = w[0];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t next = w[i + 1];
+        x[i] = __funnelshift_r(prev, next, sh);
+        prev = next;
+    }
+}
+
 // UNITS16: the row starts at a 16-byte address (which Q4_K's and Q5_K's units then do as well)
 template <int TYPE, bool UNITS16 = false>
 __device__ __forceinline__ void decode_block(const uint8_t* row, int b, uint32_t (&w)[8], float& A, float& B) {
@@ -149,6 +163,43 @@ __device__ __forceinline__ void decode_block(const uint8_t* row, int b, uint32_t
         for (int i = 0; i < 4; ++i) {
             w[i] = x[i] & 0x0F0F0F0Fu;
             w[4 + i] = (x[i] >> 4) & 0x0F0F0F0Fu;
+        }
+    }
+}
+
+// 32 consecutive values (values 32 s on) of a row: one block, or two of 16 values
+template <int TYPE, bool UNITS16 = false>
+__device__ __forceinline__ void decode32(const uint8_t* row, int s, uint32_t (&w)[8], float (&A)[32 / BlockView<TYPE>::BV],
+                                         float (&B)[32 / BlockView<TYPE>::BV]) {
+    if constexpr (TYPE == GQ_TYPE_Q6_K) {
+        const uint8_t* sp = row + 210 * (s >> 3);
+        const int h = (s >> 2) & 1, g = s & 3;
+        const float d = h2f(lds16(sp + 208));
+        const uint32_t sc = lds16(sp + 192 + 2 * (s & 7));
+        A[0] = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(sc)));
+        A[1] = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(sc >> 8)));
+        B[0] = B[1] = 0.0f;
+        uint32_t q[8];
+        load32_align2(sp + 64 * h + 32 * (g & 1), w);
+        load32_align2(sp + 128 + 32 * h, q);
+        const int lo = 4 * (g >> 1), hi = 2 * g;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = ((w[i] >> lo) & 0x0F0F0F0Fu) | (((q[i] >> hi) << 4) & 0x30303030u);
+    } else if constexpr (TYPE == GQ_TYPE_Q8_0) {
+        const uint8_t* bp = row + 34 * s;
+        A[0] = h2f(lds16(bp));
+        B[0] = 0.0f;
+        load32_align2(bp + 2, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] ^= 0x80808080u;
+    } else {
+        constexpr int NP = 32 / BlockView<TYPE>::BV, NW = BlockView<TYPE>::NW;
+#pragma unroll
+        for (int b = 0; b < NP; ++b) {
+            uint32_t x[8];
+            decode_block<TYPE, UNITS16>(row, NP * s + b, x, A[b], B[b]);
+#pragma unroll
+            for (int i = 0; i < NW; ++i) w[NW * b + i] = x[i];
         }
     }
 }

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "gq_blocks.cuh"
 #include "gq_fp8.cuh"
@@ -14,17 +15,19 @@
 namespace gq {
 namespace {
 
+// Sticky error flags of this device's weight kernels (kErrWaitTimeout).
+__device__ unsigned int gq_fp8_errors;
+
 // ---------------------------------------------------------------------------------------
 // Weights
 // ---------------------------------------------------------------------------------------
 
 // Source row of output row o (inverse of the llama q/k permutation: row 2a + t of a head
 // moves to t * D/2 + a, gguf_conversion.py:314-332).
-__device__ __forceinline__ int64_t fp8_src_row(int32_t head_dim, int64_t o) {
+__device__ __forceinline__ int64_t fp8_src_row(uint32_t head_dim, uint32_t o) {
     if (head_dim == 0) return o;
-    const int64_t h = o / head_dim;
-    const int rem = static_cast<int>(o - h * head_dim), half = head_dim >> 1;
-    const int t = rem >= half ? 1 : 0;
+    const uint32_t h = o / head_dim, rem = o - h * head_dim, half = head_dim >> 1;
+    const uint32_t t = rem >= half ? 1u : 0u;
     return h * head_dim + 2 * (rem - t * half) + t;
 }
 
@@ -36,34 +39,72 @@ struct Fp8Tile {
     static constexpr int kChunkBytes = 256 / BlockView<TYPE>::kUnitValues * BlockView<TYPE>::kUnitBytes;
     static constexpr int kChunks = ((kChunkBytes + 15 + 15) / 16) | 1;
     static constexpr int kPitch = 16 * kChunks;
-    static constexpr int kSmem = 128 * kPitch + 64;
+    static constexpr int kSmem = 128 * kPitch + 64 + 16;      // and the warps' maxima, the barrier
 };
 
-// Four codes (bytes of w, offset OFF) over the block scale as four e4m3 codes: A and B are the
-// block's constants already divided by the scale (a power of two, so every product and
-// difference rounds as before).  A byte becomes a float by placing it under the exponent of
-// 2^23 and subtracting, both exact.
+// Codes as floats by one byte permute: byte v of a word under an exponent byte is the float
+// kBase + v (v < 128 in the top mantissa bits over 2^7; 8-bit v in the middle ones over 2^15).
+// A * (v - OFF) is then one fma(A, kBase + v, -(kBase + OFF) * A), exact before its one
+// rounding because the constant is: A has at most 11 + 8 significant bits (f16 times an int8
+// or 6-bit scale; 11 where the block has no scale of its own) and kBase + OFF is 5 * 2^5
+// (Q6_K), 33 * 2^2 (Q3_K), 17 * 2^3 (Q4_0), 9 * 2^4 (Q5_0), 257 * 2^7 (Q8_0), a power of two
+// for the rest.
 template <int TYPE>
-__device__ __forceinline__ uint32_t encode_codes(uint32_t w, float A, float B) {
-    using V = BlockView<TYPE>;
-    const float2 a = make_float2(A, A), b = make_float2(-B, -B), off = make_float2(-8388608.0f - V::OFF, -8388608.0f - V::OFF);
-    uint32_t c[2];
+struct CodeFloat {
+    static constexpr bool kByte = TYPE == GQ_TYPE_Q8_0;
+    static constexpr float kBase = kByte ? 32768.0f : 128.0f;
+    static constexpr uint32_t kExp = kByte ? 0x47000000u : 0x43000000u;
+    static constexpr uint32_t kSel = kByte ? 0x7404u : 0x7044u;      // byte 0; byte k adds k at its place
+    static constexpr uint32_t kStep = kByte ? 0x0010u : 0x0100u;
+};
+
+// Four codes over the block scale as four e4m3 codes: A and B are the block's constants already
+// divided by the scale (a power of two, so every product and difference rounds as before).
+template <int TYPE>
+__device__ __forceinline__ uint32_t encode_codes(uint32_t w, float A, float C, float nB) {
+    using F = CodeFloat<TYPE>;
+    const float2 a = make_float2(A, A), c = make_float2(C, C), b = make_float2(nB, nB);
+    uint32_t r[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const float2 q = make_float2(__uint_as_float(__byte_perm(w, 0x4B000000u, 0x7650 + 2 * h)),
-                                     __uint_as_float(__byte_perm(w, 0x4B000000u, 0x7651 + 2 * h)));
-        float2 x = __fmul2_rn(a, __fadd2_rn(q, off));
-        if constexpr (V::kSub) x = __fadd2_rn(x, b);
-        c[h] = e4m3x2(x.x, x.y);
+        const float2 q = make_float2(__uint_as_float(__byte_perm(w, F::kExp, F::kSel + 2 * h * F::kStep)),
+                                     __uint_as_float(__byte_perm(w, F::kExp, F::kSel + (2 * h + 1) * F::kStep)));
+        float2 x = __ffma2_rn(a, q, c);
+        if constexpr (BlockView<TYPE>::kSub) x = __fadd2_rn(x, b);
+        r[h] = e4m3x2(x.x, x.y);
     }
-    return c[0] | (c[1] << 16);
+    return r[0] | (r[1] << 16);
 }
 
-// One CTA per 128 rows x 256 columns (two scale blocks).  A lane owns 32 consecutive columns of
-// four rows, eight lanes a row's 256: their integer codes stay in registers between the
-// block's maximum and the encoding, and a warp stores whole rows of 256 bytes.  A value is a
-// monotone function of its code, so a 16- or 32-value block's largest |x| is at its smallest or
-// largest code.
+// The largest |x| of one block as float bits: a value is a monotone function of its code, so it
+// is at the smallest or the largest code.  At or above kInfBits where a constant is not finite.
+template <int TYPE>
+__device__ __forceinline__ uint32_t block_amax(const uint32_t* w, float A, float B) {
+    using V = BlockView<TYPE>;
+    // even and odd bytes in 16-bit lanes, the odd ones left in the high halves
+    uint32_t mne = 0xFFFFFFFFu, mxe = 0u, mno = 0xFFFFFFFFu, mxo = 0u;
+#pragma unroll
+    for (int j = 0; j < V::NW; j += 2) {
+        const uint32_t e0 = w[j] & 0x00FF00FFu, e1 = w[j + 1] & 0x00FF00FFu;
+        const uint32_t o0 = w[j] & 0xFF00FF00u, o1 = w[j + 1] & 0xFF00FF00u;
+        mne = __vimin3_u16x2(mne, e0, e1);
+        mxe = __vimax3_u16x2(mxe, e0, e1);
+        mno = __vimin3_u16x2(mno, o0, o1);
+        mxo = __vimax3_u16x2(mxo, o0, o1);
+    }
+    const uint32_t mn = vmin16(mne, mno >> 8), mx = vmax16(mxe, (mxo >> 8) & 0x00FF00FFu);
+    const int lo = static_cast<int>(min(mn & 0xFFFFu, mn >> 16)) - V::OFF;
+    const int hi = static_cast<int>(max(mx & 0xFFFFu, mx >> 16)) - V::OFF;
+    if constexpr (V::kSub)
+        return max(__float_as_uint(block_value<TYPE>(A, B, lo)) & 0x7FFFFFFFu, __float_as_uint(block_value<TYPE>(A, B, hi)) & 0x7FFFFFFFu);
+    else
+        return __float_as_uint(__fmul_rn(A, static_cast<float>(max(hi, -lo)))) & 0x7FFFFFFFu;
+}
+
+// One CTA per 128 rows x 256 columns (two scale blocks).  Each row's bytes arrive by one bulk
+// copy of the aligned window around them.  A lane owns 32 consecutive columns of four rows,
+// eight lanes a row's 256: their integer codes stay in registers between the block's maximum
+// and the encoding, and a warp stores whole rows of 256 bytes.
 template <int TYPE>
 __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p) {
     using V = BlockView<TYPE>;
@@ -72,23 +113,42 @@ __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p)
     constexpr bool kUnits16 = TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K;   // 9 and 11 times 16 bytes
     extern __shared__ __align__(16) uint8_t smem[];
     uint32_t* wmax = reinterpret_cast<uint32_t*>(smem + 128 * T::kPitch);
+    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + 128 * T::kPitch + 64);
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row0 = static_cast<int64_t>(blockIdx.x / p.n_col_tiles) * 128;
-    const int64_t col0 = static_cast<int64_t>(blockIdx.x % p.n_col_tiles) * 256;
+    const uint32_t tile_r = blockIdx.x / p.n_col_tiles;
+    const uint32_t row0 = tile_r * 128;
+    const int64_t col0 = static_cast<int64_t>(blockIdx.x - tile_r * p.n_col_tiles) * 256;
     const int rows = static_cast<int>(min(static_cast<int64_t>(128), p.rows - row0));
     const int cols = static_cast<int>(min(static_cast<int64_t>(256), p.cols - col0));
     const int64_t at = col0 / V::kUnitValues * V::kUnitBytes;
     const int bytes = cols / V::kUnitValues * V::kUnitBytes;
-    for (int i = tid; i < rows * T::kChunks; i += 256) {
-        const int r = i / T::kChunks, c = i - r * T::kChunks;
-        const int64_t start = fp8_src_row(p.head_dim, row0 + r) * p.row_bytes + at;
-        const int64_t a = (start & ~int64_t(15)) + 16 * c;
-        if (a < start + bytes)
-            cp_async16(smem + r * T::kPitch + 16 * c, p.src + a, static_cast<int>(min(static_cast<int64_t>(16), p.src_bytes - a)));
+    if (tid == 0) {
+        mbar_init(bar, 128);
+        mbar_init_fence();
     }
-    cp_async_commit();
-    cp_async_wait<0>();
     __syncthreads();
+    if (tid < 128) {
+        uint32_t whole = 0;
+        const uint8_t* from = nullptr;
+        uint8_t* to = smem + tid * T::kPitch;
+        if (tid < rows) {
+            const int64_t start = fp8_src_row(p.head_dim, row0 + tid) * p.row_bytes + at, a = start & ~int64_t(15);
+            from = p.src + a;
+            whole = static_cast<uint32_t>((start + bytes - a + 15) & ~int64_t(15));
+            const int64_t left = p.src_bytes - a;
+            if (whole > left) {
+                // the tensor's last bytes, when they are no whole 16
+                whole = static_cast<uint32_t>(left) & ~15u;
+                for (int64_t i = whole; i < left; ++i) to[i] = from[i];
+            }
+        }
+        mbar_arrive_expect_tx(bar, whole);
+        if (whole != 0) bulk_load(to, from, whole, bar);
+    }
+    if (!mbar_wait(bar, 0)) {
+        atomicOr(&gq_fp8_errors, kErrWaitTimeout);
+        mbar_wait(bar, 0);     // its own copies, once more
+    }
 
     const int sub = lane & 7;
     const bool col_in = 32 * sub < cols;
@@ -102,32 +162,22 @@ __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p)
         if (!col_in || r >= rows) continue;
         int skew = 0;
         if constexpr (!kUnits16) skew = static_cast<int>((fp8_src_row(p.head_dim, row0 + r) * p.row_bytes + at) & 15);
-        const uint8_t* row = smem + r * T::kPitch + skew;
+        decode32<TYPE, kUnits16>(smem + r * T::kPitch + skew, sub, w[i], A[i], B[i]);
 #pragma unroll
         for (int b = 0; b < NP; ++b) {
-            uint32_t words[8];
-            decode_block<TYPE, kUnits16>(row, NP * sub + b, words, A[i][b], B[i][b]);
-#pragma unroll
-            for (int j = 0; j < V::NW; ++j) w[i][V::NW * b + j] = words[j];
-            if ((__float_as_uint(A[i][b]) & 0x7FFFFFFFu) < kInfBits && (__float_as_uint(B[i][b]) & 0x7FFFFFFFu) < kInfBits) {
-                uint32_t mn = 0xFFFFFFFFu, mx = 0u;
-#pragma unroll
-                for (int j = 0; j < V::NW; ++j) {
-                    const uint32_t e = words[j] & 0x00FF00FFu, o = (words[j] >> 8) & 0x00FF00FFu;
-                    mn = vmin16(mn, e, o);
-                    mx = vmax16(mx, e, o);
-                }
-                const int lo = static_cast<int>(min(mn & 0xFFFFu, mn >> 16)) - V::OFF;
-                const int hi = static_cast<int>(max(mx & 0xFFFFu, mx >> 16)) - V::OFF;
-                amax = max(amax, max(finite_abs(block_value<TYPE>(A[i][b], B[i][b], lo)),
-                                     finite_abs(block_value<TYPE>(A[i][b], B[i][b], hi))));
-            } else {
+            uint32_t m = block_amax<TYPE>(w[i] + V::NW * b, A[i][b], B[i][b]);
+            if (m >= kInfBits) {
                 finite = false;
+                m = 0;
                 for (int j = 0; j < V::BV; ++j) {
-                    const int q = static_cast<int>(byte_of(words[j >> 2], j & 3)) - V::OFF;
-                    amax = max(amax, finite_abs(block_value<TYPE>(A[i][b], B[i][b], q)));
+                    const uint32_t word = j < 16 ? (j < 8 ? (j < 4 ? w[i][V::NW * b] : w[i][V::NW * b + 1])
+                                                          : (j < 12 ? w[i][V::NW * b + 2] : w[i][V::NW * b + 3]))
+                                                 : (j < 24 ? (j < 20 ? w[i][4] : w[i][5]) : (j < 28 ? w[i][6] : w[i][7]));
+                    const int q = static_cast<int>((word >> (8 * (j & 3))) & 0xFFu) - V::OFF;
+                    m = max(m, finite_abs(block_value<TYPE>(A[i][b], B[i][b], q)));
                 }
             }
+            amax = max(amax, m);
         }
     }
     // lanes with equal bit 2 hold the same block's columns
@@ -142,8 +192,9 @@ __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p)
     const uint32_t byte = scale_byte(max(max(max(m0.x, m0.y), max(m0.z, m0.w)), max(max(m1.x, m1.y), max(m1.z, m1.w))));
     const float inv = inverse_scale(byte);
     if (warp == 0 && (lane & 27) == 0 && 128 * half < cols)
-        p.scales[(row0 >> 7) * p.scale_cols + (col0 >> 7) + half] = static_cast<uint8_t>(byte);
+        p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + (col0 >> 7) + half] = static_cast<uint8_t>(byte);
     const bool sectors = (reinterpret_cast<uintptr_t>(p.codes) & 31) == 0;    // rows are multiples of 32 bytes
+    constexpr float kAll = CodeFloat<TYPE>::kBase + static_cast<float>(V::OFF);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int r = 32 * i + 4 * warp + (lane >> 3);
@@ -151,8 +202,11 @@ __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p)
         uint32_t c[8];
         if (finite) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
-                c[j] = encode_codes<TYPE>(w[i][j], __fmul_rn(A[i][j / V::NW], inv), V::kSub ? __fmul_rn(B[i][j / V::NW], inv) : 0.0f);
+            for (int b = 0; b < NP; ++b) {
+                const float a = __fmul_rn(A[i][b], inv), k = __fmul_rn(a, -kAll), nb = V::kSub ? -__fmul_rn(B[i][b], inv) : 0.0f;
+#pragma unroll
+                for (int j = 0; j < V::NW; ++j) c[V::NW * b + j] = encode_codes<TYPE>(w[i][V::NW * b + j], a, k, nb);
+            }
         } else {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -190,11 +244,6 @@ struct Elem<F32> {
         x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
         x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
     }
-    static __device__ __forceinline__ float round(float x) { return x; }
-    static __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
-        stg128f(reinterpret_cast<float*>(p), x[0], x[1], x[2], x[3]);
-        stg128f(reinterpret_cast<float*>(p) + 4, x[4], x[5], x[6], x[7]);
-    }
 };
 template <>
 struct Elem<F16> {
@@ -207,14 +256,6 @@ struct Elem<F16> {
             x[2 * i] = h2f(w[i]);
             x[2 * i + 1] = h2f(w[i] >> 16);
         }
-    }
-    static __device__ __forceinline__ float round(float x) { return __half2float(__float2half_rn(x)); }
-    static __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = __half_as_ushort(__float2half_rn(x[2 * i])) | (static_cast<uint32_t>(__half_as_ushort(__float2half_rn(x[2 * i + 1]))) << 16);
-        stg128(p, make_uint4(w[0], w[1], w[2], w[3]));
     }
 };
 template <>
@@ -229,27 +270,15 @@ struct Elem<BF16> {
             x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
         }
     }
-    static __device__ __forceinline__ float round(float x) { return __bfloat162float(__float2bfloat16_rn(x)); }
-    static __device__ __forceinline__ void store8(void* p, const float (&x)[8]) {
-        uint32_t w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            w[i] = __bfloat16_as_ushort(__float2bfloat16_rn(x[2 * i])) |
-                   (static_cast<uint32_t>(__bfloat16_as_ushort(__float2bfloat16_rn(x[2 * i + 1]))) << 16);
-        stg128(p, make_uint4(w[0], w[1], w[2], w[3]));
-    }
 };
 
-// Eight values over the block scale to eight codes.  A NaN becomes the NaN code by itself; an
-// infinity would saturate, so callers that may hold one make it a NaN first (SAFE).
-template <bool SAFE>
+// Eight values over the block scale to eight codes
 __device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv) {
     uint32_t c[4];
     const float2 s = make_float2(inv, inv);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        const float u = SAFE ? x[2 * i] : nan_unless_finite(x[2 * i]), v = SAFE ? x[2 * i + 1] : nan_unless_finite(x[2 * i + 1]);
-        const float2 y = __fmul2_rn(make_float2(u, v), s);
+        const float2 y = __fmul2_rn(make_float2(nan_unless_finite(x[2 * i]), nan_unless_finite(x[2 * i + 1])), s);
         c[i] = e4m3x2(y.x, y.y);
     }
     return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
@@ -259,30 +288,6 @@ __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
 #pragma unroll
     for (int k = 0; k < 8; ++k) m = max(m, finite_abs(x[k]));
     return m;
-}
-// the largest |x| with NaN left out (fmaxf does) and infinities in
-__device__ __forceinline__ float amax8_or_inf(const float (&x)[8]) {
-    const float a = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
-    const float b = fmaxf(fmaxf(fabsf(x[4]), fabsf(x[5])), fmaxf(fabsf(x[6]), fabsf(x[7])));
-    return fmaxf(a, b);
-}
-// over the 16 lanes that hold one 128-value block
-__device__ __forceinline__ uint32_t max16(uint32_t m) {
-#pragma unroll
-    for (int d = 8; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
-    return m;
-}
-
-// The codes and scale byte of one 128-value block by 16 lanes, eight values each; all lanes
-// of the warp call it together.
-__device__ __forceinline__ uint2 quantize_block(const float (&x)[8], uint32_t& byte) {
-    uint32_t m = max16(__float_as_uint(amax8_or_inf(x)));   // non-negative floats order as their bits
-    if (__any_sync(0xffffffffu, m >= kInfBits)) {
-        byte = scale_byte(max16(amax8(x)));
-        return encode8<false>(x, inverse_scale(byte));
-    }
-    byte = scale_byte(m);
-    return encode8<true>(x, inverse_scale(byte));
 }
 
 // Weights of a float type: one CTA per 128 x 128 block, thread t the 8 columns 8 (t % 16) of
@@ -299,7 +304,7 @@ __global__ void __launch_bounds__(256) gq_fp8_float_weight_kernel(const GqFp8Wei
     for (int i = 0; i < 8; ++i) {
         const int64_t r = row0 + (tid >> 4) + 16 * i;
         if (r < p.rows && col < p.cols) {
-            Elem<T>::load8(p.src + fp8_src_row(p.head_dim, r) * p.row_bytes + col * Elem<T>::kBytes, x[i]);
+            Elem<T>::load8(p.src + fp8_src_row(p.head_dim, static_cast<uint32_t>(r)) * p.row_bytes + col * Elem<T>::kBytes, x[i]);
             amax = max(amax, amax8(x[i]));
         }
     }
@@ -315,7 +320,7 @@ __global__ void __launch_bounds__(256) gq_fp8_float_weight_kernel(const GqFp8Wei
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const int64_t r = row0 + (tid >> 4) + 16 * i;
-        if (r < p.rows && col < p.cols) st_global(reinterpret_cast<uint2*>(p.codes + r * p.cols + col), encode8<false>(x[i], inv));
+        if (r < p.rows && col < p.cols) st_global(reinterpret_cast<uint2*>(p.codes + r * p.cols + col), encode8(x[i], inv));
     }
 }
 
@@ -341,178 +346,335 @@ int launch_float_weight(GqFp8Weight& p, cudaStream_t s) {
 }
 
 // ---------------------------------------------------------------------------------------
-// Activations
+// Activations: 16 consecutive values per lane, eight lanes per 128-value block
 // ---------------------------------------------------------------------------------------
 
-// y = silu(g) * x = g / (1 + exp(-g)) * x, or x.  The reciprocal and the exponential are the
-// hardware's approximations (a few ulp of f32, where a code keeps 4 bits); g = -inf gives NaN
-// and a g whose exponential overflows gives -0, as the formula does.
-template <bool GATED>
-__device__ __forceinline__ void gate8(float (&x)[8], const float (&g)[8]) {
-    if constexpr (GATED) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-            float r;
-            asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, __expf(-g[k]))));
-            x[k] = __fmul_rn(__fmul_rn(g[k], r), x[k]);
-        }
-    }
-}
+// 16 values as they lie in memory.  Rows start on 16-byte boundaries; where they start on 32
+// (WIDE, the same for a whole launch) one load takes 32 bytes.
+template <class T>
+struct Raw16 {
+    static constexpr int kWords = 4 * Elem<T>::kBytes;
+    uint32_t w[kWords];
 
-// Rows as they are or gated: a block per 16 lanes, kSteps blocks per lane with all their loads
-// ahead of the arithmetic.  Blocks are numbered through the rows (fewer than 2^31 per launch).
-constexpr int kSteps = 2;
-template <class T, bool GATED>
-__global__ void __launch_bounds__(256) gq_fp8_rows_kernel(const GqFp8Rows p, const uint32_t count, const uint32_t mul,
-                                                          const uint32_t shift) {
-    constexpr int E = Elem<T>::kBytes;
-    const uint32_t sub = threadIdx.x & 15;
-    const uint32_t first = blockIdx.x * (16 * kSteps) + (threadIdx.x >> 4);
-    uint32_t row[kSteps], col[kSteps];
-    bool in[kSteps];
-    float x[kSteps][8], g[GATED ? kSteps : 1][8];
+    __device__ __forceinline__ void load(const uint8_t* p, bool wide) {
+        if (wide) {
 #pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        const uint32_t b = first + 16 * i;
-        row[i] = fast_div(b, mul, shift);
-        col[i] = 128 * (b - row[i] * static_cast<uint32_t>(p.blocks)) + 8 * sub;
-        in[i] = b < count && col[i] < p.cols;
-#pragma unroll
-        for (int k = 0; k < 8; ++k) x[i][k] = 0.0f;
-        if constexpr (GATED)
-#pragma unroll
-            for (int k = 0; k < 8; ++k) g[i][k] = 0.0f;
-        if (in[i]) {
-            Elem<T>::load8(p.x + (row[i] * p.ld_x + col[i]) * E, x[i]);
-            if constexpr (GATED) Elem<T>::load8(p.gate + (row[i] * p.ld_gate + col[i]) * E, g[i]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i) {
-        gate8<GATED>(x[i], g[GATED ? i : 0]);
-        uint32_t byte;
-        const uint2 c = quantize_block(x[i], byte);
-        if (in[i]) {
-            st_global(reinterpret_cast<uint2*>(p.codes + row[i] * p.ld_codes + col[i]), c);
-            if (sub == 0) p.scales[row[i] * p.ld_scales + (col[i] >> 7)] = static_cast<uint8_t>(byte);
-        }
-    }
-}
-
-// RMS norm of a row (with the residual's addition), one CTA per row: h stays in registers
-// between the sum of squares and the codes (VPT groups of eight values per thread; 0: rows too
-// long for that are read again).  The sum x + r is rounded to the input type first: the norm
-// is of what the next layer reads.
-template <class T, bool RESIDUAL, int VPT>
-__global__ void __launch_bounds__(1024) gq_fp8_norm_kernel(const GqFp8Rows p) {
-    constexpr int E = Elem<T>::kBytes;
-    __shared__ float wsum[32];
-    const int64_t row = blockIdx.x;
-    const int tid = threadIdx.x, threads = blockDim.x;
-    const uint8_t* xr = p.x + row * p.ld_x * E;
-    const uint8_t* rr = RESIDUAL ? p.residual + row * p.ld_residual * E : nullptr;
-    uint8_t* hr = RESIDUAL ? p.sum + row * p.ld_sum * E : nullptr;
-    const auto add = [&](float (&h)[8], const float (&r)[8], int64_t c) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) h[k] = Elem<T>::round(__fadd_rn(h[k], r[k]));
-        Elem<T>::store8(hr + c * E, h);
-    };
-    const auto squares = [](const float (&h)[8], float s) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) s = __fmaf_rn(h[k], h[k], s);
-        return s;
-    };
-    float h[VPT > 0 ? VPT : 1][8];
-    float ss = 0.0f;
-    if constexpr (VPT > 0) {
-        float r[VPT][8];
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = 8 * (tid + i * threads);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) h[i][k] = 0.0f;
-            if (c < p.cols) {
-                Elem<T>::load8(xr + c * E, h[i]);
-                if constexpr (RESIDUAL) Elem<T>::load8(rr + c * E, r[i]);
-            }
-        }
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) {
-            const int64_t c = 8 * (tid + i * threads);
-            if constexpr (RESIDUAL)
-                if (c < p.cols) add(h[i], r[i], c);
-            ss = squares(h[i], ss);
-        }
-    } else {
-        for (int64_t c = 8 * tid; c < p.cols; c += 8 * threads) {
-            Elem<T>::load8(xr + c * E, h[0]);
-            if constexpr (RESIDUAL) {
-                float r[8];
-                Elem<T>::load8(rr + c * E, r);
-                add(h[0], r, c);
-            }
-            ss = squares(h[0], ss);
-        }
-    }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
-    if (threads > 32) {
-        if ((tid & 31) == 0) wsum[tid >> 5] = ss;
-        __syncthreads();
-        ss = (tid & 31) < (threads >> 5) ? wsum[tid & 31] : 0.0f;
-#pragma unroll
-        for (int d = 16; d > 0; d >>= 1) ss = __fadd_rn(ss, __shfl_xor_sync(0xffffffffu, ss, d));
-    }
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, static_cast<float>(p.cols)), p.eps)));
-    const auto finish = [&](float (&y)[8], int64_t c) {
-        const bool in = c < p.cols;
-        if (in) {
-            float w[8];
-            Elem<F32>::load8(p.weight + c, w);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = __fmul_rn(__fmul_rn(y[k], rstd), w[k]);
+            for (int i = 0; i < kWords; i += 8)
+                asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3]), "=r"(w[i + 4]), "=r"(w[i + 5]),
+                               "=r"(w[i + 6]), "=r"(w[i + 7])
+                             : "l"(p + 4 * i));
         } else {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) y[k] = 0.0f;
-        }
-        uint32_t byte;
-        const uint2 codes = quantize_block(y, byte);
-        if (in) {
-            st_global(reinterpret_cast<uint2*>(p.codes + row * p.ld_codes + c), codes);
-            if ((tid & 15) == 0) p.scales[row * p.ld_scales + (c >> 7)] = static_cast<uint8_t>(byte);
-        }
-    };
-    if constexpr (VPT > 0) {
-#pragma unroll
-        for (int i = 0; i < VPT; ++i) finish(h[i], 8 * (tid + i * threads));
-    } else {
-        for (int64_t c0 = 0; c0 < p.cols; c0 += 8 * threads) {   // all lanes together (quantize_block)
-            const int64_t c = c0 + 8 * tid;
-            if (c < p.cols) Elem<T>::load8((RESIDUAL ? hr : xr) + c * E, h[0]);   // this thread wrote these values itself
-            finish(h[0], c);
+            for (int i = 0; i < kWords; i += 4)
+                asm volatile("ld.global.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                             : "l"(p + 4 * i));
         }
     }
+    __device__ __forceinline__ void store(uint8_t* p, bool wide) const {
+#pragma unroll
+        for (int i = 0; i < kWords; i += 8) {
+            if (wide) {
+                const uint32_t v[8] = {w[i], w[i + 1], w[i + 2], w[i + 3], w[i + 4], w[i + 5], w[i + 6], w[i + 7]};
+                stg256(p + 4 * i, v);
+            } else {
+                stg128(p + 4 * i, make_uint4(w[i], w[i + 1], w[i + 2], w[i + 3]));
+                stg128(p + 4 * i + 16, make_uint4(w[i + 4], w[i + 5], w[i + 6], w[i + 7]));
+            }
+        }
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = 0;
+    }
+    // value pair i of 8
+    __device__ __forceinline__ float2 get(int i) const {
+        if constexpr (std::is_same<T, F32>::value) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+        else if constexpr (std::is_same<T, F16>::value) return __half22float2(u32_as_h2(w[i]));
+        else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+    }
+    // rounds to the type
+    __device__ __forceinline__ void set(int i, float2 v) {
+        if constexpr (std::is_same<T, F32>::value) {
+            w[2 * i] = __float_as_uint(v.x);
+            w[2 * i + 1] = __float_as_uint(v.y);
+        } else if constexpr (std::is_same<T, F16>::value) {
+            const __half2 h = __float22half2_rn(v);
+            memcpy(&w[i], &h, 4);
+        } else {
+            const __nv_bfloat162 h = __float22bfloat162_rn(v);
+            memcpy(&w[i], &h, 4);
+        }
+    }
+};
+
+// over the eight lanes that hold one 128-value block
+__device__ __forceinline__ uint32_t max8(uint32_t m) {
+#pragma unroll
+    for (int d = 4; d > 0; d >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, d));
+    return m;
+}
+
+// The codes and scale byte of one 128-value block by eight lanes, 16 values each; all lanes of
+// the warp call it together.  fmaxf leaves NaN out, and NaN becomes its code by itself; an
+// infinity shows in the maximum, and then the values are looked at one by one.
+__device__ __forceinline__ uint4 quantize_block(float2 (&y)[8], uint32_t& byte) {
+    float m[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        m[i] = fmaxf(fmaxf(fabsf(y[2 * i].x), fabsf(y[2 * i].y)), fmaxf(fabsf(y[2 * i + 1].x), fabsf(y[2 * i + 1].y)));
+    // non-negative floats order as their bits
+    uint32_t amax = max8(__float_as_uint(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]))));
+    if (__any_sync(0xffffffffu, amax >= kInfBits)) {
+        amax = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            amax = max(amax, max(finite_abs(y[i].x), finite_abs(y[i].y)));
+            y[i] = make_float2(nan_unless_finite(y[i].x), nan_unless_finite(y[i].y));
+        }
+        amax = max8(amax);
+    }
+    byte = scale_byte(amax);
+    const float inv = inverse_scale(byte);
+    const float2 s = make_float2(inv, inv);
+    uint32_t c[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 u = __fmul2_rn(y[2 * i], s), v = __fmul2_rn(y[2 * i + 1], s);
+        c[i] = e4m3x2(u.x, u.y) | (e4m3x2(v.x, v.y) << 16);
+    }
+    return make_uint4(c[0], c[1], c[2], c[3]);
+}
+
+// silu(g) * x = g / (1 + exp(-g)) * x.  The reciprocal and the exponential are the hardware's
+// approximations (a few ulp of f32, where a code keeps 4 bits); g = -inf gives NaN and a g
+// whose exponential overflows gives -0, as the formula does.
+__device__ __forceinline__ float silu_times(float g, float x) {
+    float e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(__fmul_rn(g, -1.4426950408889634f)));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(__fadd_rn(1.0f, e)));
+    return __fmul_rn(__fmul_rn(g, r), x);
+}
+
+// Rows as they are or gated, a block per eight lanes.  Blocks are numbered through the rows
+// (fewer than 2^31 per launch).
+template <class T, bool GATED>
+__global__ void __launch_bounds__(256) gq_fp8_rows_kernel(const GqFp8Rows p, const uint32_t count, const uint32_t mul,
+                                                          const uint32_t shift, const bool wide) {
+    constexpr int E = Elem<T>::kBytes;
+    const uint32_t sub = threadIdx.x & 7;
+    const uint32_t b = blockIdx.x * 32 + (threadIdx.x >> 3);
+    const uint32_t row = fast_div(b, mul, shift);
+    const uint32_t kb = b - row * static_cast<uint32_t>(p.blocks), col = 128 * kb + 16 * sub;
+    const bool in = b < count && col < p.cols;
+    Raw16<T> x, g;
+    x.clear();
+    if constexpr (GATED) g.clear();
+    if (in) {
+        x.load(p.x + (row * p.ld_x + col) * E, wide);
+        if constexpr (GATED) g.load(p.gate + (row * p.ld_gate + col) * E, wide);
+    }
+    float2 y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        y[i] = x.get(i);
+        if constexpr (GATED) {
+            const float2 v = g.get(i);
+            y[i] = make_float2(silu_times(v.x, y[i].x), silu_times(v.y, y[i].y));
+        }
+    }
+    uint32_t byte;
+    const uint4 c = quantize_block(y, byte);
+    if (in) {
+        stg128(p.codes + row * p.ld_codes + col, c);
+        if (sub == 0) p.scales[row * p.ld_scales + kb] = static_cast<uint8_t>(byte);
+    }
+}
+
+// RMS norm of rows (with the residual's addition): a CTA takes rows one after another, each
+// lane NV groups of 16 values of every row.  h stays in registers between the sum of squares
+// and the codes; with one group per lane the weights stay there too and the next row's loads
+// are issued before this row's sum is joined.  The sum x + r is rounded to the input type
+// first: the norm is of what the next layer reads.
+template <class T, bool RESIDUAL, int NV>
+__global__ void __launch_bounds__(512) gq_fp8_norm_kernel(const GqFp8Rows p, const bool wide) {
+    constexpr int E = Elem<T>::kBytes;
+    __shared__ float wsum[2][16];
+    const int tid = threadIdx.x, threads = blockDim.x;
+    const auto column = [&](int i) { return 16 * (static_cast<int64_t>(tid) + static_cast<int64_t>(i) * threads); };
+    const auto fetch = [&](int64_t row, int i, Raw16<T>& x, Raw16<T>& r) {
+        const int64_t c = column(i);
+        x.clear();
+        if constexpr (RESIDUAL) r.clear();
+        if (row < p.rows && c < p.cols) {
+            x.load(p.x + (row * p.ld_x + c) * E, wide);
+            if constexpr (RESIDUAL) r.load(p.residual + (row * p.ld_residual + c) * E, wide);
+        }
+    };
+    float4 weight[NV == 1 ? 4 : 1];
+    if constexpr (NV == 1) {
+        if (column(0) < p.cols)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) weight[j] = reinterpret_cast<const float4*>(p.weight + column(0))[j];
+    }
+    Raw16<T> x[NV], r[RESIDUAL ? NV : 1];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) fetch(blockIdx.x, i, x[i], r[RESIDUAL ? i : 0]);
+    int turn = 0;
+    for (int64_t row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+        Raw16<T> h[NV];
+        float2 ss = make_float2(0.0f, 0.0f);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                if constexpr (RESIDUAL) h[i].set(k, __fadd2_rn(x[i].get(k), r[i].get(k)));
+                const float2 v = RESIDUAL ? h[i].get(k) : x[i].get(k);
+                ss = __ffma2_rn(v, v, ss);
+            }
+            if constexpr (RESIDUAL) {
+                if (column(i) < p.cols) h[i].store(p.sum + (row * p.ld_sum + column(i)) * E, wide);
+            } else {
+                h[i] = x[i];
+            }
+        }
+        if constexpr (NV == 1) fetch(row + gridDim.x, 0, x[0], r[0]);
+        float s = __fadd_rn(ss.x, ss.y);
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, d));
+        if (threads > 32) {
+            if ((tid & 31) == 0) wsum[turn][tid >> 5] = s;
+            __syncthreads();
+            s = (tid & 15) < (threads >> 5) ? wsum[turn][tid & 15] : 0.0f;
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, d));
+        }
+        const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, static_cast<float>(p.cols)), p.eps)));
+        const float2 rs = make_float2(rstd, rstd);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            const int64_t c = column(i);
+            const bool in = c < p.cols;
+            float2 y[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float4 w = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                if constexpr (NV == 1) w = weight[j];
+                else if (in) w = reinterpret_cast<const float4*>(p.weight + c)[j];
+                y[2 * j] = __fmul2_rn(__fmul2_rn(h[i].get(2 * j), rs), make_float2(w.x, w.y));
+                y[2 * j + 1] = __fmul2_rn(__fmul2_rn(h[i].get(2 * j + 1), rs), make_float2(w.z, w.w));
+            }
+            if (!in)
+#pragma unroll
+                for (int k = 0; k < 8; ++k) y[k] = make_float2(0.0f, 0.0f);
+            uint32_t byte;
+            const uint4 codes = quantize_block(y, byte);
+            if (in) {
+                stg128(p.codes + row * p.ld_codes + c, codes);
+                if ((tid & 7) == 0) p.scales[row * p.ld_scales + (c >> 7)] = static_cast<uint8_t>(byte);
+            }
+        }
+        if constexpr (NV > 1)
+#pragma unroll
+            for (int i = 0; i < NV; ++i) fetch(row + gridDim.x, i, x[i], r[RESIDUAL ? i : 0]);
+    }
+}
+
+// Rows too long for registers: the sum of squares in one pass, the codes in another that reads
+// h again.
+template <class T, bool RESIDUAL>
+__global__ void __launch_bounds__(512) gq_fp8_long_norm_kernel(const GqFp8Rows p, const bool wide) {
+    constexpr int E = Elem<T>::kBytes;
+    __shared__ float wsum[16];
+    const int tid = threadIdx.x;
+    const int64_t row = blockIdx.x;
+    const uint8_t* from = p.x + row * p.ld_x * E;
+    float2 ss = make_float2(0.0f, 0.0f);
+    for (int64_t c = 16 * tid; c < p.cols; c += 16 * 512) {
+        Raw16<T> x;
+        x.load(from + c * E, wide);
+        if constexpr (RESIDUAL) {
+            Raw16<T> r;
+            r.load(p.residual + (row * p.ld_residual + c) * E, wide);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) x.set(k, __fadd2_rn(x.get(k), r.get(k)));
+            x.store(p.sum + (row * p.ld_sum + c) * E, wide);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) ss = __ffma2_rn(x.get(k), x.get(k), ss);
+    }
+    float s = __fadd_rn(ss.x, ss.y);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, d));
+    if ((tid & 31) == 0) wsum[tid >> 5] = s;
+    __syncthreads();
+    s = wsum[tid & 15];
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) s = __fadd_rn(s, __shfl_xor_sync(0xffffffffu, s, d));
+    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(s, static_cast<float>(p.cols)), p.eps)));
+    if constexpr (RESIDUAL) from = p.sum + row * p.ld_sum * E;      // what this thread wrote itself
+    for (int64_t c0 = 0; c0 < p.cols; c0 += 16 * 512) {           // all lanes together (quantize_block)
+        const int64_t c = c0 + 16 * tid;
+        const bool in = c < p.cols;
+        float2 y[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) y[k] = make_float2(0.0f, 0.0f);
+        if (in) {
+            Raw16<T> h;
+            h.load(from + c * E, wide);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const float2 w = reinterpret_cast<const float2*>(p.weight + c)[k], v = h.get(k);
+                y[k] = make_float2(__fmul_rn(__fmul_rn(v.x, rstd), w.x), __fmul_rn(__fmul_rn(v.y, rstd), w.y));
+            }
+        }
+        uint32_t byte;
+        const uint4 codes = quantize_block(y, byte);
+        if (in) {
+            stg128(p.codes + row * p.ld_codes + c, codes);
+            if ((tid & 7) == 0) p.scales[row * p.ld_scales + (c >> 7)] = static_cast<uint8_t>(byte);
+        }
+    }
+}
+
+template <class T, bool RESIDUAL, int NV>
+void launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
+    auto kern = gq_fp8_norm_kernel<T, RESIDUAL, NV>;
+    const int threads = static_cast<int>(((p.cols + 15) / 16 + 32 * NV - 1) / (32 * NV) * 32);
+    int dev = 0, sms = 0, per = 0;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    int64_t grid = p.rows;
+    if (grid > sms) {
+        cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, 0);
+        grid = std::min<int64_t>(grid, static_cast<int64_t>(sms) * std::max(per, 1));
+    }
+    kern<<<static_cast<unsigned>(grid), threads, 0, s>>>(p, wide);
 }
 
 template <class T, bool RESIDUAL>
-void launch_norm(const GqFp8Rows& p, cudaStream_t s) {
-    const int64_t eights = (p.cols + 7) / 8;
-    const auto threads = [&](int vpt) { return static_cast<unsigned>((eights + 32 * vpt - 1) / (32 * vpt) * 32); };
-    const unsigned rows = static_cast<unsigned>(p.rows);
-    if (eights <= 512) gq_fp8_norm_kernel<T, RESIDUAL, 1><<<rows, threads(1), 0, s>>>(p);
-    else if (eights <= 1024) gq_fp8_norm_kernel<T, RESIDUAL, 2><<<rows, threads(2), 0, s>>>(p);
-    else if (eights <= 4096) gq_fp8_norm_kernel<T, RESIDUAL, 4><<<rows, threads(4), 0, s>>>(p);
-    else gq_fp8_norm_kernel<T, RESIDUAL, 0><<<rows, 1024, 0, s>>>(p);
+void launch_norm(const GqFp8Rows& p, bool wide, cudaStream_t s) {
+    if (p.cols <= 8192) launch_norm_rows<T, RESIDUAL, 1>(p, wide, s);
+    else if (p.cols <= 16384) launch_norm_rows<T, RESIDUAL, 2>(p, wide, s);
+    else gq_fp8_long_norm_kernel<T, RESIDUAL><<<static_cast<unsigned>(p.rows), 512, 0, s>>>(p, wide);
+}
+
+// every row starts on a 32-byte boundary
+bool rows32(const void* p, int64_t ld, int64_t rows, int elem_bytes) {
+    return p == nullptr || ((reinterpret_cast<uintptr_t>(p) & 31) == 0 && (rows <= 1 || (ld * elem_bytes) % 32 == 0));
 }
 
 template <class T>
 int launch_rows(GqFp8Rows p, cudaStream_t s) {
+    constexpr int E = Elem<T>::kBytes;
+    const bool wide = rows32(p.x, p.ld_x, p.rows, E) && rows32(p.gate, p.ld_gate, p.rows, E) &&
+                      rows32(p.residual, p.ld_residual, p.rows, E) && rows32(p.sum, p.ld_sum, p.rows, E);
     if (p.weight != nullptr) {
-        if (p.residual != nullptr) launch_norm<T, true>(p, s);
-        else launch_norm<T, false>(p, s);
+        if (p.residual != nullptr) launch_norm<T, true>(p, wide, s);
+        else launch_norm<T, false>(p, wide, s);
         return static_cast<int>(cudaGetLastError());
     }
-    if (p.blocks > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     uint32_t mul, shift;
     fast_div_params(static_cast<uint32_t>(p.blocks), mul, shift);
     // rows in runs of fewer than 2^31 blocks
@@ -520,11 +682,10 @@ int launch_rows(GqFp8Rows p, cudaStream_t s) {
     for (int64_t r = 0; r < all; r += run) {
         p.rows = std::min(run, all - r);
         const uint32_t count = static_cast<uint32_t>(p.rows * p.blocks);
-        const unsigned grid = (count + 16 * kSteps - 1) / (16 * kSteps);
-        if (p.gate != nullptr) gq_fp8_rows_kernel<T, true><<<grid, 256, 0, s>>>(p, count, mul, shift);
-        else gq_fp8_rows_kernel<T, false><<<grid, 256, 0, s>>>(p, count, mul, shift);
-        p.x += run * p.ld_x * Elem<T>::kBytes;
-        if (p.gate != nullptr) p.gate += run * p.ld_gate * Elem<T>::kBytes;
+        if (p.gate != nullptr) gq_fp8_rows_kernel<T, true><<<(count + 31) / 32, 256, 0, s>>>(p, count, mul, shift, wide);
+        else gq_fp8_rows_kernel<T, false><<<(count + 31) / 32, 256, 0, s>>>(p, count, mul, shift, wide);
+        p.x += run * p.ld_x * E;
+        if (p.gate != nullptr) p.gate += run * p.ld_gate * E;
         p.codes += run * p.ld_codes;
         p.scales += run * p.ld_scales;
     }
@@ -551,6 +712,17 @@ int launch_fp8_weight(int type, GqFp8Weight& p, void* stream) {
         case GQ_TYPE_Q6_K: return launch_weight<GQ_TYPE_Q6_K>(p, s);
         default: return static_cast<int>(cudaErrorInvalidValue);
     }
+}
+
+int fp8_errors(bool clear, uint32_t* flags) {
+    unsigned v = 0;
+    cudaError_t e = cudaMemcpyFromSymbol(&v, gq_fp8_errors, sizeof(v));
+    if (e == cudaSuccess && clear && v != 0) {
+        const unsigned zero = 0;
+        e = cudaMemcpyToSymbol(gq_fp8_errors, &zero, sizeof(zero));
+    }
+    *flags = v;
+    return static_cast<int>(e);
 }
 
 int launch_fp8_rows(int dtype, const GqFp8Rows& p, void* stream) {

@@ -105,7 +105,7 @@ struct GqFp8Weight {
     int64_t rows, cols;
     int64_t row_bytes, src_bytes;   // of the GGUF tensor
     int64_t scale_cols;
-    int32_t head_dim;         // > 0: llama q/k head permutation with heads of this size
+    uint32_t head_dim;        // > 0: llama q/k head permutation with heads of this size
     uint32_t n_col_tiles;     // set by the launch
 };
 
@@ -142,6 +142,8 @@ struct GqMatmul {
 int launch_fp8_weight(int type, GqFp8Weight& p, void* stream);
 int launch_fp8_rows(int dtype, const GqFp8Rows& p, void* stream);
 int launch_matmul(int dtype, const GqMatmul& p, void* stream);
-int matmul_errors(bool clear, uint32_t* flags);   // as kernel_errors, of the product kernels
+// as kernel_errors, of the kernels of these two files
+int fp8_errors(bool clear, uint32_t* flags);
+int matmul_errors(bool clear, uint32_t* flags);
 
 }  // namespace gq

@@ -39,25 +39,26 @@ struct BlockView {
                                                              : 210;
 };
 
+// 32 bytes as eight words from `bits` bits after (before, if negative) a shared address that is a
+// multiple of 2: a shift that the fields of the words need costs nothing beside the one that the
+// alignment needs.  Bits that come in from neighbouring bytes are the caller's to mask.
+__device__ __forceinline__ void load32_bits(const uint8_t* p, int bits, uint32_t (&x)[8]) {
+    const uint32_t a = 8u * smem_u32addr(p) + static_cast<uint32_t>(bits);     // shared addresses fit in 18 bits
+    const uint32_t sh = a & 31u, w = (a >> 5) << 2;
+    uint32_t prev = lds_u32(w);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const uint32_t next = lds_u32(w + 4 * i + 4);
+        x[i] = __funnelshift_r(prev, next, sh);
+        prev = next;
+    }
+}
+
 // 16 bytes of a unit: rows of 16-byte units at 16-byte addresses (UNITS16) in one load
 template <bool UNITS16>
 __device__ __forceinline__ uint4 unit_bytes16(const uint8_t* p) {
     if constexpr (UNITS16) return lds128(p);
     else return lds128_align2(p);
-}
-
-// 32 bytes at a 2-byte-aligned shared address as eight words
-__device__ __forceinline__ void load32_align2(const uint8_t* p, uint32_t (&x)[8]) {
-    const uintptr_t a = reinterpret_cast<uintptr_t>(p);
-    const uint32_t* w = reinterpret_cast<const uint32_t*>(a & ~uintptr_t(3));
-    const uint32_t sh = static_cast<uint32_t>(a & 3u) * 8u;
-    uint32_t prev = w[0];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const uint32_t next = w[i + 1];
-        x[i] = __funnelshift_r(prev, next, sh);
-        prev = next;
-    }
 }
 
 // UNITS16: the row starts at a 16-byte address (which Q4_K's and Q5_K's units then do as well)
@@ -179,17 +180,17 @@ __device__ __forceinline__ void decode32(const uint8_t* row, int s, uint32_t (&w
         A[0] = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(sc)));
         A[1] = __fmul_rn(d, static_cast<float>(static_cast<int8_t>(sc >> 8)));
         B[0] = B[1] = 0.0f;
+        // low nibbles or high ones of 32 bytes, and bits 2g.. of 32 more moved to bits 4 and 5
         uint32_t q[8];
-        load32_align2(sp + 64 * h + 32 * (g & 1), w);
-        load32_align2(sp + 128 + 32 * h, q);
-        const int lo = 4 * (g >> 1), hi = 2 * g;
+        load32_bits(sp + 64 * h + 32 * (g & 1), 4 * (g >> 1), w);
+        load32_bits(sp + 128 + 32 * h, 2 * g - 4, q);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = ((w[i] >> lo) & 0x0F0F0F0Fu) | (((q[i] >> hi) << 4) & 0x30303030u);
+        for (int i = 0; i < 8; ++i) w[i] = (w[i] & 0x0F0F0F0Fu) | (q[i] & 0x30303030u);
     } else if constexpr (TYPE == GQ_TYPE_Q8_0) {
         const uint8_t* bp = row + 34 * s;
         A[0] = h2f(lds16(bp));
         B[0] = 0.0f;
-        load32_align2(bp + 2, w);
+        load32_bits(bp + 2, 0, w);
 #pragma unroll
         for (int i = 0; i < 8; ++i) w[i] ^= 0x80808080u;
     } else {

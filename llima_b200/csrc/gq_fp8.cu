@@ -11,6 +11,7 @@
 #include "gq_blocks.cuh"
 #include "gq_fp8.cuh"
 #include "gq_internal.h"
+#include "gq_launch.h"
 
 namespace gq {
 namespace {
@@ -31,108 +32,127 @@ __device__ __forceinline__ int64_t fp8_src_row(uint32_t head_dim, uint32_t o) {
     return h * head_dim + 2 * (rem - t * half) + t;
 }
 
-// Shared bytes per row of a 256-column tile: the 16-byte-aligned window around the row's
-// bytes, an odd number of 16-byte chunks so that lanes on neighbouring rows read different
-// banks.
+// A tile is 128 rows x 256 columns, two scale blocks.  Shared bytes per row: the 16-byte-aligned
+// window around the row's bytes, an odd number of 16-byte chunks so that lanes on neighbouring
+// rows read different banks.
 template <int TYPE>
 struct Fp8Tile {
+    static constexpr int kThreads = 512;
+    static constexpr int kStages = 2;
     static constexpr int kChunkBytes = 256 / BlockView<TYPE>::kUnitValues * BlockView<TYPE>::kUnitBytes;
-    static constexpr int kChunks = ((kChunkBytes + 15 + 15) / 16) | 1;
-    static constexpr int kPitch = 16 * kChunks;
-    static constexpr int kSmem = 128 * kPitch + 64 + 16;      // and the warps' maxima, the barrier
+    static constexpr int kPitch = 16 * (((kChunkBytes + 15 + 15) / 16) | 1);
+    static constexpr int kStageBytes = 128 * kPitch + 16;      // decoding may read a word past a row
+    static constexpr int kSmem = kStages * kStageBytes + kStages * 8 + 3 * 2 * 4;
+    static constexpr int kPerSm = 2;
 };
 
-// Codes as floats by one byte permute: byte v of a word under an exponent byte is the float
-// kBase + v (v < 128 in the top mantissa bits over 2^7; 8-bit v in the middle ones over 2^15).
-// A * (v - OFF) is then one fma(A, kBase + v, -(kBase + OFF) * A), exact before its one
-// rounding because the constant is: A has at most 11 + 8 significant bits (f16 times an int8
-// or 6-bit scale; 11 where the block has no scale of its own) and kBase + OFF is 5 * 2^5
-// (Q6_K), 33 * 2^2 (Q3_K), 17 * 2^3 (Q4_0), 9 * 2^4 (Q5_0), 257 * 2^7 (Q8_0), a power of two
-// for the rest.
+// One 16- or 32-value block's codes as f16 pairs (exact) ...
 template <int TYPE>
-struct CodeFloat {
-    static constexpr bool kByte = TYPE == GQ_TYPE_Q8_0;
-    static constexpr float kBase = kByte ? 32768.0f : 128.0f;
-    static constexpr uint32_t kExp = kByte ? 0x47000000u : 0x43000000u;
-    static constexpr uint32_t kSel = kByte ? 0x7404u : 0x7044u;      // byte 0; byte k adds k at its place
-    static constexpr uint32_t kStep = kByte ? 0x0010u : 0x0100u;
-};
-
-// Four codes over the block scale as four e4m3 codes: A and B are the block's constants already
-// divided by the scale (a power of two, so every product and difference rounds as before).
-template <int TYPE>
-__device__ __forceinline__ uint32_t encode_codes(uint32_t w, float A, float C, float nB) {
-    using F = CodeFloat<TYPE>;
-    const float2 a = make_float2(A, A), c = make_float2(C, C), b = make_float2(nB, nB);
-    uint32_t r[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const float2 q = make_float2(__uint_as_float(__byte_perm(w, F::kExp, F::kSel + 2 * h * F::kStep)),
-                                     __uint_as_float(__byte_perm(w, F::kExp, F::kSel + (2 * h + 1) * F::kStep)));
-        float2 x = __ffma2_rn(a, q, c);
-        if constexpr (BlockView<TYPE>::kSub) x = __fadd2_rn(x, b);
-        r[h] = e4m3x2(x.x, x.y);
-    }
-    return r[0] | (r[1] << 16);
-}
-
-// The largest |x| of one block as float bits: a value is a monotone function of its code, so it
-// is at the smallest or the largest code.  At or above kInfBits where a constant is not finite.
-template <int TYPE>
-__device__ __forceinline__ uint32_t block_amax(const uint32_t* w, float A, float B) {
+__device__ __forceinline__ void codes_to_half(const uint32_t* w, __half2* q) {
     using V = BlockView<TYPE>;
-    // even and odd bytes in 16-bit lanes, the odd ones left in the high halves
-    uint32_t mne = 0xFFFFFFFFu, mxe = 0u, mno = 0xFFFFFFFFu, mxo = 0u;
+    // a byte under the exponent byte of 1024 is the f16 1024 + v
+    const __half2 off = __float2half2_rn(-1024.0f - V::OFF);
 #pragma unroll
-    for (int j = 0; j < V::NW; j += 2) {
-        const uint32_t e0 = w[j] & 0x00FF00FFu, e1 = w[j + 1] & 0x00FF00FFu;
-        const uint32_t o0 = w[j] & 0xFF00FF00u, o1 = w[j + 1] & 0xFF00FF00u;
-        mne = __vimin3_u16x2(mne, e0, e1);
-        mxe = __vimax3_u16x2(mxe, e0, e1);
-        mno = __vimin3_u16x2(mno, o0, o1);
-        mxo = __vimax3_u16x2(mxo, o0, o1);
+    for (int j = 0; j < V::NW; ++j) {
+        q[2 * j] = __hadd2_rn(u32_as_h2(__byte_perm(w[j], 0x64646464u, 0x4140)), off);
+        q[2 * j + 1] = __hadd2_rn(u32_as_h2(__byte_perm(w[j], 0x64646464u, 0x4342)), off);
     }
-    const uint32_t mn = vmin16(mne, mno >> 8), mx = vmax16(mxe, (mxo >> 8) & 0x00FF00FFu);
-    const int lo = static_cast<int>(min(mn & 0xFFFFu, mn >> 16)) - V::OFF;
-    const int hi = static_cast<int>(max(mx & 0xFFFFu, mx >> 16)) - V::OFF;
-    if constexpr (V::kSub)
-        return max(__float_as_uint(block_value<TYPE>(A, B, lo)) & 0x7FFFFFFFu, __float_as_uint(block_value<TYPE>(A, B, hi)) & 0x7FFFFFFFu);
-    else
-        return __float_as_uint(__fmul_rn(A, static_cast<float>(max(hi, -lo)))) & 0x7FFFFFFFu;
 }
 
-// One CTA per 128 rows x 256 columns (two scale blocks).  Each row's bytes arrive by one bulk
-// copy of the aligned window around them.  A lane owns 32 consecutive columns of four rows,
-// eight lanes a row's 256: their integer codes stay in registers between the block's maximum
-// and the encoding, and a warp stores whole rows of 256 bytes.
+// ... and its largest |x| as float bits: a value is a monotone function of its code, so it is at
+// the smallest or the largest code.  At or above kInfBits where a constant is not finite.
 template <int TYPE>
-__global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p) {
+__device__ __forceinline__ uint32_t block_amax(const __half2* q, float A, float B) {
+    using V = BlockView<TYPE>;
+    if constexpr (V::kSub) {
+        __half2 mn = q[0], mx = q[0];
+#pragma unroll
+        for (int j = 1; j < 2 * V::NW; ++j) {
+            mn = __hmin2(mn, q[j]);
+            mx = __hmax2(mx, q[j]);
+        }
+        const float lo = __half2float(__hmin(__low2half(mn), __high2half(mn)));
+        const float hi = __half2float(__hmax(__low2half(mx), __high2half(mx)));
+        return max(__float_as_uint(__fsub_rn(__fmul_rn(A, lo), B)) & 0x7FFFFFFFu,
+                   __float_as_uint(__fsub_rn(__fmul_rn(A, hi), B)) & 0x7FFFFFFFu);
+    } else {
+        uint32_t m;
+        memcpy(&m, &q[0], 4);
+#pragma unroll
+        for (int j = 1; j < 2 * V::NW; ++j) {
+            uint32_t x;
+            memcpy(&x, &q[j], 4);
+            asm("max.xorsign.abs.f16x2 %0, %0, %1;" : "+r"(m) : "r"(x));   // magnitudes; the signs mean nothing
+        }
+        const float hi = fmaxf(fabsf(h2f(m)), fabsf(h2f(m >> 16)));
+        return __float_as_uint(__fmul_rn(A, hi)) & 0x7FFFFFFFu;
+    }
+}
+
+// One x of a code's f16 value, as gguf-py computes it
+template <int TYPE>
+__device__ __forceinline__ float half_value(float A, float B, __half q) {
+    const float x = __fmul_rn(A, __half2float(q));
+    return BlockView<TYPE>::kSub ? __fsub_rn(x, B) : x;
+}
+
+// 32 codes over the block scale as e4m3.  The constants are divided by the scale, a power of two,
+// so that every product and difference rounds as before.
+template <int TYPE, bool CHECK>
+__device__ __forceinline__ void encode32(const __half2* q, const float* A, const float* B, float inv, uint32_t (&c)[8]) {
+    using V = BlockView<TYPE>;
+#pragma unroll
+    for (int b = 0; b < 32 / V::BV; ++b) {
+        const float a = __fmul_rn(A[b], inv), nb = V::kSub ? -__fmul_rn(B[b], inv) : 0.0f;
+        const float2 a2 = make_float2(a, a), nb2 = make_float2(nb, nb);
+#pragma unroll
+        for (int j = V::NW * b; j < V::NW * (b + 1); ++j) {
+            float2 x = __fmul2_rn(a2, __half22float2(q[2 * j])), y = __fmul2_rn(a2, __half22float2(q[2 * j + 1]));
+            if constexpr (V::kSub) {
+                x = __fadd2_rn(x, nb2);
+                y = __fadd2_rn(y, nb2);
+            }
+            if constexpr (CHECK) {
+                x = make_float2(nan_unless_finite(x.x), nan_unless_finite(x.y));
+                y = make_float2(nan_unless_finite(y.x), nan_unless_finite(y.y));
+            }
+            c[j] = e4m3x2(x.x, x.y) | (e4m3x2(y.x, y.y) << 16);
+        }
+    }
+}
+
+// A persistent grid of CTAs with a ring of two tiles each: a row's bytes arrive by one bulk copy
+// of the aligned window around them, two tiles ahead.  A lane owns 32 consecutive columns of two
+// rows, eight lanes a row's 256: their codes stay in registers between the block's maximum and
+// the encoding (and the stage is free for the next copy), and a warp stores whole rows of 256
+// bytes.  The arithmetic is placed on the half-rate integer pipe as little as possible: codes
+// become f16 pairs by one permute and one add, the maximum is taken two at a time.
+template <int TYPE>
+__global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm) gq_fp8_weight_kernel(const GqFp8Weight p) {
     using V = BlockView<TYPE>;
     using T = Fp8Tile<TYPE>;
-    constexpr int NP = 32 / V::BV;                                          // blocks per 32 columns
+    constexpr int NP = 32 / V::BV, NR = 2;                                  // blocks per 32 columns, rows per lane
     constexpr bool kUnits16 = TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K;   // 9 and 11 times 16 bytes
     extern __shared__ __align__(16) uint8_t smem[];
-    uint32_t* wmax = reinterpret_cast<uint32_t*>(smem + 128 * T::kPitch);
-    uint64_t* bar = reinterpret_cast<uint64_t*>(smem + 128 * T::kPitch + 64);
+    uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kStages * T::kStageBytes);
+    uint32_t* wmax = reinterpret_cast<uint32_t*>(bars + T::kStages);     // [turn % 3][half]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const uint32_t tile_r = blockIdx.x / p.n_col_tiles;
-    const uint32_t row0 = tile_r * 128;
-    const int64_t col0 = static_cast<int64_t>(blockIdx.x - tile_r * p.n_col_tiles) * 256;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(128), p.rows - row0));
-    const int cols = static_cast<int>(min(static_cast<int64_t>(256), p.cols - col0));
-    const int64_t at = col0 / V::kUnitValues * V::kUnitBytes;
-    const int bytes = cols / V::kUnitValues * V::kUnitBytes;
     if (tid == 0) {
-        mbar_init(bar, 128);
+        for (int s = 0; s < T::kStages; ++s) mbar_init(bars + s, 128);
         mbar_init_fence();
+        for (int i = 0; i < 6; ++i) wmax[i] = 0;
     }
     __syncthreads();
-    if (tid < 128) {
+    const auto issue = [&](uint32_t t, int s) {      // threads 0..127: one row each
+        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift);
+        const int64_t col0 = static_cast<int64_t>(t - tile_r * p.n_col_tiles) * 256;
+        const int64_t at = col0 / V::kUnitValues * V::kUnitBytes;
+        const int64_t bytes = min(static_cast<int64_t>(256), p.cols - col0) / V::kUnitValues * V::kUnitBytes;
         uint32_t whole = 0;
         const uint8_t* from = nullptr;
-        uint8_t* to = smem + tid * T::kPitch;
-        if (tid < rows) {
-            const int64_t start = fp8_src_row(p.head_dim, row0 + tid) * p.row_bytes + at, a = start & ~int64_t(15);
+        uint8_t* to = smem + s * T::kStageBytes + tid * T::kPitch;
+        if (tile_r * 128 + tid < p.rows) {
+            const int64_t start = fp8_src_row(p.head_dim, tile_r * 128 + tid) * p.row_bytes + at, a = start & ~int64_t(15);
             from = p.src + a;
             whole = static_cast<uint32_t>((start + bytes - a + 15) & ~int64_t(15));
             const int64_t left = p.src_bytes - a;
@@ -142,90 +162,102 @@ __global__ void __launch_bounds__(256) gq_fp8_weight_kernel(const GqFp8Weight p)
                 for (int64_t i = whole; i < left; ++i) to[i] = from[i];
             }
         }
-        mbar_arrive_expect_tx(bar, whole);
-        if (whole != 0) bulk_load(to, from, whole, bar);
-    }
-    if (!mbar_wait(bar, 0)) {
-        atomicOr(&gq_fp8_errors, kErrWaitTimeout);
-        mbar_wait(bar, 0);     // its own copies, once more
-    }
+        mbar_arrive_expect_tx(bars + s, whole);
+        if (whole != 0) bulk_load(to, from, whole, bars + s);
+    };
+    if (tid < 128)
+        for (int s = 0; s < T::kStages; ++s)
+            if (blockIdx.x + s * gridDim.x < p.n_tiles) issue(blockIdx.x + s * gridDim.x, s);
 
-    const int sub = lane & 7;
-    const bool col_in = 32 * sub < cols;
-    uint32_t w[4][8];
-    float A[4][NP], B[4][NP];
-    uint32_t amax = 0;
-    bool finite = true;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 32 * i + 4 * warp + (lane >> 3);
-        if (!col_in || r >= rows) continue;
-        int skew = 0;
-        if constexpr (!kUnits16) skew = static_cast<int>((fp8_src_row(p.head_dim, row0 + r) * p.row_bytes + at) & 15);
-        decode32<TYPE, kUnits16>(smem + r * T::kPitch + skew, sub, w[i], A[i], B[i]);
-#pragma unroll
-        for (int b = 0; b < NP; ++b) {
-            uint32_t m = block_amax<TYPE>(w[i] + V::NW * b, A[i][b], B[i][b]);
-            if (m >= kInfBits) {
-                finite = false;
-                m = 0;
-                for (int j = 0; j < V::BV; ++j) {
-                    const uint32_t word = j < 16 ? (j < 8 ? (j < 4 ? w[i][V::NW * b] : w[i][V::NW * b + 1])
-                                                          : (j < 12 ? w[i][V::NW * b + 2] : w[i][V::NW * b + 3]))
-                                                 : (j < 24 ? (j < 20 ? w[i][4] : w[i][5]) : (j < 28 ? w[i][6] : w[i][7]));
-                    const int q = static_cast<int>((word >> (8 * (j & 3))) & 0xFFu) - V::OFF;
-                    m = max(m, finite_abs(block_value<TYPE>(A[i][b], B[i][b], q)));
-                }
-            }
-            amax = max(amax, m);
-        }
-    }
-    // lanes with equal bit 2 hold the same block's columns
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
-    amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
-    const int half = (lane >> 2) & 1;
-    if ((lane & 27) == 0) wmax[8 * half + warp] = amax;
-    __syncthreads();
-    const uint4 m0 = *reinterpret_cast<const uint4*>(wmax + 8 * half), m1 = *reinterpret_cast<const uint4*>(wmax + 8 * half + 4);
-    const uint32_t byte = scale_byte(max(max(max(m0.x, m0.y), max(m0.z, m0.w)), max(max(m1.x, m1.y), max(m1.z, m1.w))));
-    const float inv = inverse_scale(byte);
-    if (warp == 0 && (lane & 27) == 0 && 128 * half < cols)
-        p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + (col0 >> 7) + half] = static_cast<uint8_t>(byte);
+    const int sub = lane & 7, half = (lane >> 2) & 1;
     const bool sectors = (reinterpret_cast<uintptr_t>(p.codes) & 31) == 0;    // rows are multiples of 32 bytes
-    constexpr float kAll = CodeFloat<TYPE>::kBase + static_cast<float>(V::OFF);
+    uint32_t n = 0;
+    for (uint32_t t = blockIdx.x; t < p.n_tiles; t += gridDim.x, ++n) {
+        const int s = n % T::kStages;
+        if (!mbar_wait(bars + s, (n / T::kStages) & 1)) {
+            atomicOr(&gq_fp8_errors, kErrWaitTimeout);
+            break;
+        }
+        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift), row0 = tile_r * 128;
+        const int64_t col0 = static_cast<int64_t>(t - tile_r * p.n_col_tiles) * 256;
+        const int rows = static_cast<int>(min(static_cast<int64_t>(128), p.rows - row0));
+        const int cols = static_cast<int>(min(static_cast<int64_t>(256), p.cols - col0));
+        const bool col_in = 32 * sub < cols;
+        __half2 q[NR][16];
+        float A[NR][NP], B[NR][NP];
+        uint32_t amax = 0;
+        bool finite = true;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = 32 * i + 4 * warp + (lane >> 3);
-        if (!col_in || r >= rows) continue;
-        uint32_t c[8];
-        if (finite) {
+        for (int i = 0; i < NR; ++i) {
+            const int r = 64 * i + 4 * warp + (lane >> 3);
+            if (!col_in || r >= rows) continue;
+            int skew = 0;
+            if constexpr (!kUnits16)
+                skew = static_cast<int>((static_cast<uint32_t>(fp8_src_row(p.head_dim, row0 + r)) * static_cast<uint32_t>(p.row_bytes) +
+                                         static_cast<uint32_t>(col0) / V::kUnitValues * V::kUnitBytes) & 15u);
+            uint32_t w[8];
+            decode32<TYPE, kUnits16>(smem + s * T::kStageBytes + r * T::kPitch + skew, sub, w, A[i], B[i]);
 #pragma unroll
             for (int b = 0; b < NP; ++b) {
-                const float a = __fmul_rn(A[i][b], inv), k = __fmul_rn(a, -kAll), nb = V::kSub ? -__fmul_rn(B[i][b], inv) : 0.0f;
+                codes_to_half<TYPE>(w + V::NW * b, q[i] + 2 * V::NW * b);
+                uint32_t m = block_amax<TYPE>(q[i] + 2 * V::NW * b, A[i][b], B[i][b]);
+                if (m >= kInfBits) {
+                    finite = false;
+                    m = 0;
 #pragma unroll
-                for (int j = 0; j < V::NW; ++j) c[V::NW * b + j] = encode_codes<TYPE>(w[i][V::NW * b + j], a, k, nb);
-            }
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float x[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    x[k] = __fmul_rn(nan_unless_finite(block_value<TYPE>(A[i][j / V::NW], B[i][j / V::NW],
-                                                                         static_cast<int>(byte_of(w[i][j], k)) - V::OFF)), inv);
-                c[j] = e4m3x2(x[0], x[1]) | (e4m3x2(x[2], x[3]) << 16);
+                    for (int j = 0; j < 2 * V::NW; ++j) {
+                        const __half2 v = q[i][2 * V::NW * b + j];
+                        m = max(m, max(finite_abs(half_value<TYPE>(A[i][b], B[i][b], __low2half(v))),
+                                       finite_abs(half_value<TYPE>(A[i][b], B[i][b], __high2half(v)))));
+                    }
+                }
+                amax = max(amax, m);
             }
         }
-        uint8_t* out = p.codes + (row0 + r) * p.cols + col0 + 32 * sub;
-        if (sectors) {
-            stg256(out, c);
-        } else {
-            stg128(out, make_uint4(c[0], c[1], c[2], c[3]));
-            stg128(out + 16, make_uint4(c[4], c[5], c[6], c[7]));
+        // lanes with equal bit 2 hold the same block's columns
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 8));
+        amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
+        // joined over the warps in one of three places in turn; the next turn's is cleared here,
+        // after its last reading and before its next use
+        uint32_t* const wm = wmax + 2 * (n % 3) + half;
+        if ((lane & 27) == 0) {
+            atomicMax(wm, amax);
+            if (warp == 0) wmax[2 * ((n + 1) % 3) + half] = 0;
+        }
+        __syncthreads();
+        // every thread is done with the stage
+        if (tid < 128 && t + T::kStages * gridDim.x < p.n_tiles) issue(t + T::kStages * gridDim.x, s);
+        amax = *wm;
+        const uint32_t byte = scale_byte(amax);
+        const float inv = inverse_scale(byte);
+        if (warp == 0 && (lane & 27) == 0 && 128 * half < cols)
+            p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + (col0 >> 7) + half] = static_cast<uint8_t>(byte);
+        // a warp with a value that is not finite takes its own way
+        const bool plain = __all_sync(0xffffffffu, finite);
+#pragma unroll
+        for (int i = 0; i < NR; ++i) {
+            const int r = 64 * i + 4 * warp + (lane >> 3);
+            if (!col_in || r >= rows) continue;
+            uint32_t c[8];
+            if (plain) encode32<TYPE, false>(q[i], A[i], B[i], inv, c);
+            else encode32<TYPE, true>(q[i], A[i], B[i], inv, c);
+            uint8_t* out = p.codes + (static_cast<int64_t>(row0) + r) * p.cols + col0 + 32 * sub;
+            if (sectors) {
+                stg256(out, c);
+            } else {
+                stg128(out, make_uint4(c[0], c[1], c[2], c[3]));
+                stg128(out + 16, make_uint4(c[4], c[5], c[6], c[7]));
+            }
         }
     }
+    // after a wait that gave up, nothing of this CTA stays in flight
+    if (static_cast<uint64_t>(blockIdx.x) + static_cast<uint64_t>(n) * gridDim.x < p.n_tiles)
+        for (int s = 0; s < T::kStages; ++s) {
+            const uint64_t t = blockIdx.x + static_cast<uint64_t>(n + s) * gridDim.x;
+            if (t < p.n_tiles) mbar_wait(bars + (n + s) % T::kStages, ((n + s) / T::kStages) & 1);
+        }
 }
 
 // ---- elements of the float types, eight at a time -----------------------------------------
@@ -328,13 +360,14 @@ template <int TYPE>
 int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     using T = Fp8Tile<TYPE>;
     auto kern = gq_fp8_weight_kernel<TYPE>;
-    if (T::kSmem > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
-        if (e != cudaSuccess) return static_cast<int>(e);
-    }
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = allow_smem(kern, T::kSmem, allowed);
+    if (e != cudaSuccess) return static_cast<int>(e);
     p.n_col_tiles = static_cast<uint32_t>((p.cols + 255) / 256);
-    const int64_t tiles = (p.rows + 127) / 128 * p.n_col_tiles;
-    kern<<<static_cast<unsigned>(tiles), 256, T::kSmem, s>>>(p);
+    p.n_tiles = static_cast<uint32_t>((p.rows + 127) / 128 * p.n_col_tiles);
+    fast_div_params(p.n_col_tiles, p.ncol_mul, p.ncol_shift);
+    const uint32_t most = static_cast<uint32_t>(sm_count() * T::kPerSm);
+    kern<<<std::min(p.n_tiles, most), T::kThreads, T::kSmem, s>>>(p);
     return static_cast<int>(cudaGetLastError());
 }
 template <class T>
@@ -642,9 +675,8 @@ template <class T, bool RESIDUAL, int NV>
 void launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
     auto kern = gq_fp8_norm_kernel<T, RESIDUAL, NV>;
     const int threads = static_cast<int>(((p.cols + 15) / 16 + 32 * NV - 1) / (32 * NV) * 32);
-    int dev = 0, sms = 0, per = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    const int sms = sm_count();
+    int per = 0;
     int64_t grid = p.rows;
     if (grid > sms) {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, 0);

@@ -14,9 +14,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
-#include <atomic>
-
 #include "gq_internal.h"
+#include "gq_launch.h"
 #include "gq_tcgen05.cuh"
 
 namespace gq {
@@ -526,26 +525,6 @@ bool tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, step,
               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-int sm_count() {
-    int dev = 0, sms = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms;
-}
-
-// The kernel's shared memory limit, raised once per device and kernel (`done`: a bit per device).
-template <class K>
-cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
-    int dev = 0;
-    const cudaError_t g = cudaGetDevice(&dev);
-    if (g != cudaSuccess) return g;
-    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
-    if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_release);
-    return e;
 }
 
 template <int BN, class T>

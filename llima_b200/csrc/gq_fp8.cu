@@ -12,6 +12,7 @@
 #include "gq_fp8.cuh"
 #include "gq_internal.h"
 #include "gq_launch.h"
+#include "gq_tcgen05.cuh"
 
 namespace gq {
 namespace {
@@ -41,7 +42,7 @@ struct Fp8Tile {
     static constexpr int kStages = 2;
     static constexpr int kChunkBytes = 256 / BlockView<TYPE>::kUnitValues * BlockView<TYPE>::kUnitBytes;
     static constexpr int kPitch = 16 * (((kChunkBytes + 15 + 15) / 16) | 1);
-    static constexpr int kStageBytes = 128 * kPitch + 16;      // decoding may read a word past a row
+    static constexpr int kStageBytes = 128 * kPitch + 128;     // decoding may read a word past a row
     static constexpr int kSmem = kStages * kStageBytes + kStages * 8 + 3 * 2 * 4;
     static constexpr int kPerSm = 2;
 };
@@ -96,6 +97,16 @@ __device__ __forceinline__ float half_value(float A, float B, __half q) {
     return BlockView<TYPE>::kSub ? __fsub_rn(x, B) : x;
 }
 
+// The largest finite |x| of a block whose constants are not all finite
+template <int TYPE>
+__device__ __forceinline__ uint32_t finite_amax(const __half2* q, float A, float B) {
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 2 * BlockView<TYPE>::NW; ++j)
+        m = max(m, max(finite_abs(half_value<TYPE>(A, B, __low2half(q[j]))), finite_abs(half_value<TYPE>(A, B, __high2half(q[j])))));
+    return m;
+}
+
 // 32 codes over the block scale as e4m3.  The constants are divided by the scale, a power of two,
 // so that every product and difference rounds as before.
 template <int TYPE, bool CHECK>
@@ -121,41 +132,65 @@ __device__ __forceinline__ void encode32(const __half2* q, const float* A, const
     }
 }
 
-// A persistent grid of CTAs with a ring of two tiles each: a row's bytes arrive by one bulk copy
-// of the aligned window around them, two tiles ahead.  A lane owns 32 consecutive columns of two
+// A persistent grid of CTAs with a ring of two tiles each, loaded two tiles ahead.  BOXES: the
+// rows' windows arrive as boxes of a tensor map (columns of 4 bytes, the two rows of a permuted
+// pair, pairs), issued by one thread; p.box_rows rows to a box.  That takes rows of whole 16
+// bytes, and heads whose half is 8, 16, 32 or 64 rows or a multiple of 128.  Otherwise every row's
+// window is a bulk copy of its own, which costs a loop over lanes (28 against 26 us for Q6_K
+// 4096 x 14336).  A lane owns 32 consecutive columns of two
 // rows, eight lanes a row's 256: their codes stay in registers between the block's maximum and
 // the encoding (and the stage is free for the next copy), and a warp stores whole rows of 256
 // bytes.  The arithmetic is placed on the half-rate integer pipe as little as possible: codes
 // become f16 pairs by one permute and one add, the maximum is taken two at a time.
-template <int TYPE>
-__global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm) gq_fp8_weight_kernel(const GqFp8Weight p) {
+template <int TYPE, bool BOXES>
+__global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm) gq_fp8_weight_kernel(
+    const __grid_constant__ CUtensorMap map, const GqFp8Weight p) {
     using V = BlockView<TYPE>;
     using T = Fp8Tile<TYPE>;
     constexpr int NP = 32 / V::BV, NR = 2;                                  // blocks per 32 columns, rows per lane
     constexpr bool kUnits16 = TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K;   // 9 and 11 times 16 bytes
-    extern __shared__ __align__(16) uint8_t smem[];
+    extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kStages * T::kStageBytes);
     uint32_t* wmax = reinterpret_cast<uint32_t*>(bars + T::kStages);     // [turn % 3][half]
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
-        for (int s = 0; s < T::kStages; ++s) mbar_init(bars + s, 128);
+        for (int s = 0; s < T::kStages; ++s) mbar_init(bars + s, BOXES ? 1 : 128);
         mbar_init_fence();
         for (int i = 0; i < 6; ++i) wmax[i] = 0;
     }
     __syncthreads();
-    const auto issue = [&](uint32_t t, int s) {      // threads 0..127: one row each
-        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift);
-        const int64_t col0 = static_cast<int64_t>(t - tile_r * p.n_col_tiles) * 256;
-        const int64_t at = col0 / V::kUnitValues * V::kUnitBytes;
-        const int64_t bytes = min(static_cast<int64_t>(256), p.cols - col0) / V::kUnitValues * V::kUnitBytes;
+    const uint32_t all_rows = static_cast<uint32_t>(p.rows), all_cols = static_cast<uint32_t>(p.cols);
+    constexpr uint32_t kColBytes = T::kChunkBytes;         // of 256 columns
+    const auto issue = [&](uint32_t t, int s) {
+        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift), tile_c = t - tile_r * p.n_col_tiles;
+        if constexpr (BOXES) {
+            if (warp == 0 && tc::elect()) {
+                const uint32_t bar = smem_u32addr(bars + s), x = tile_c * kColBytes / 16 * 4;
+                tc::arrive_expect(bar, 128 * T::kPitch);
+                for (uint32_t r = 0; r < 128; r += p.box_rows) {
+                    uint32_t o = tile_r * 128 + r, second = 0;
+                    if (p.head_dim != 0) {
+                        const uint32_t h = o / p.head_dim, rem = o - h * p.head_dim, hd = p.head_dim >> 1;
+                        second = rem >= hd ? 1u : 0u;
+                        o = h * hd + rem - second * hd;
+                    }
+                    tc::load_box(smem_u32addr(smem + s * T::kStageBytes + r * T::kPitch), &map, static_cast<int>(x),
+                                 static_cast<int>(second), static_cast<int>(o), bar);
+                }
+            }
+            return;
+        }
+        if (tid >= 128) return;                      // one row each
+        const uint32_t bytes = min(256u, all_cols - 256 * tile_c) / V::kUnitValues * V::kUnitBytes;
         uint32_t whole = 0;
         const uint8_t* from = nullptr;
         uint8_t* to = smem + s * T::kStageBytes + tid * T::kPitch;
-        if (tile_r * 128 + tid < p.rows) {
-            const int64_t start = fp8_src_row(p.head_dim, tile_r * 128 + tid) * p.row_bytes + at, a = start & ~int64_t(15);
-            from = p.src + a;
-            whole = static_cast<uint32_t>((start + bytes - a + 15) & ~int64_t(15));
-            const int64_t left = p.src_bytes - a;
+        if (tile_r * 128 + tid < all_rows) {
+            const int64_t start = fp8_src_row(p.head_dim, tile_r * 128 + tid) * p.row_bytes + static_cast<int64_t>(tile_c) * kColBytes;
+            const uint32_t skew = static_cast<uint32_t>(start) & 15u;
+            from = p.src + (start - skew);
+            whole = (skew + bytes + 15u) & ~15u;
+            const int64_t left = p.src_bytes - (start - skew);
             if (whole > left) {
                 // the tensor's last bytes, when they are no whole 16
                 whole = static_cast<uint32_t>(left) & ~15u;
@@ -165,51 +200,46 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
         mbar_arrive_expect_tx(bars + s, whole);
         if (whole != 0) bulk_load(to, from, whole, bars + s);
     };
-    if (tid < 128)
-        for (int s = 0; s < T::kStages; ++s)
-            if (blockIdx.x + s * gridDim.x < p.n_tiles) issue(blockIdx.x + s * gridDim.x, s);
+    for (int s = 0; s < T::kStages; ++s)
+        if (blockIdx.x + s * gridDim.x < p.n_tiles) issue(blockIdx.x + s * gridDim.x, s);
 
     const int sub = lane & 7, half = (lane >> 2) & 1;
     const bool sectors = (reinterpret_cast<uintptr_t>(p.codes) & 31) == 0;    // rows are multiples of 32 bytes
+    // what does not change from tile to tile: this lane's first row and its place in the output
+    const uint32_t my_row = 4 * warp + (lane >> 3);
+    uint8_t* const my_out = p.codes + static_cast<int64_t>(my_row) * p.cols + 32 * sub;
+    const uint8_t* const my_smem = smem + my_row * T::kPitch;
+    const uint32_t row_bytes16 = static_cast<uint32_t>(p.row_bytes) & 15u;
     uint32_t n = 0;
+    int s = 0;
+    uint32_t parity = 0, turn = 0;
     for (uint32_t t = blockIdx.x; t < p.n_tiles; t += gridDim.x, ++n) {
-        const int s = n % T::kStages;
-        if (!mbar_wait(bars + s, (n / T::kStages) & 1)) {
+        if (!mbar_wait(bars + s, parity)) {
             atomicOr(&gq_fp8_errors, kErrWaitTimeout);
             break;
         }
-        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift), row0 = tile_r * 128;
-        const int64_t col0 = static_cast<int64_t>(t - tile_r * p.n_col_tiles) * 256;
-        const int rows = static_cast<int>(min(static_cast<int64_t>(128), p.rows - row0));
-        const int cols = static_cast<int>(min(static_cast<int64_t>(256), p.cols - col0));
-        const bool col_in = 32 * sub < cols;
+        const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift), tile_c = t - tile_r * p.n_col_tiles;
+        const uint32_t row0 = tile_r * 128, rows = all_rows - row0, cols = all_cols - 256 * tile_c;    // left from here on
+        const bool col_in = static_cast<uint32_t>(32 * sub) < cols;
         __half2 q[NR][16];
         float A[NR][NP], B[NR][NP];
         uint32_t amax = 0;
         bool finite = true;
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
-            const int r = 64 * i + 4 * warp + (lane >> 3);
-            if (!col_in || r >= rows) continue;
-            int skew = 0;
+            if (!col_in || my_row + 64 * i >= rows) continue;
+            uint32_t skew = 0;
             if constexpr (!kUnits16)
-                skew = static_cast<int>((static_cast<uint32_t>(fp8_src_row(p.head_dim, row0 + r)) * static_cast<uint32_t>(p.row_bytes) +
-                                         static_cast<uint32_t>(col0) / V::kUnitValues * V::kUnitBytes) & 15u);
+                skew = (static_cast<uint32_t>(fp8_src_row(p.head_dim, row0 + my_row + 64 * i)) * row_bytes16 + tile_c * kColBytes) & 15u;
             uint32_t w[8];
-            decode32<TYPE, kUnits16>(smem + s * T::kStageBytes + r * T::kPitch + skew, sub, w, A[i], B[i]);
+            decode32<TYPE, kUnits16>(my_smem + s * T::kStageBytes + 64 * i * T::kPitch + skew, sub, w, A[i], B[i]);
 #pragma unroll
             for (int b = 0; b < NP; ++b) {
                 codes_to_half<TYPE>(w + V::NW * b, q[i] + 2 * V::NW * b);
                 uint32_t m = block_amax<TYPE>(q[i] + 2 * V::NW * b, A[i][b], B[i][b]);
                 if (m >= kInfBits) {
                     finite = false;
-                    m = 0;
-#pragma unroll
-                    for (int j = 0; j < 2 * V::NW; ++j) {
-                        const __half2 v = q[i][2 * V::NW * b + j];
-                        m = max(m, max(finite_abs(half_value<TYPE>(A[i][b], B[i][b], __low2half(v))),
-                                       finite_abs(half_value<TYPE>(A[i][b], B[i][b], __high2half(v)))));
-                    }
+                    m = finite_amax<TYPE>(q[i] + 2 * V::NW * b, A[i][b], B[i][b]);
                 }
                 amax = max(amax, m);
             }
@@ -221,29 +251,32 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
         amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, 16));
         // joined over the warps in one of three places in turn; the next turn's is cleared here,
         // after its last reading and before its next use
-        uint32_t* const wm = wmax + 2 * (n % 3) + half;
+        uint32_t* const wm = wmax + 2 * turn + half;
+        turn = turn == 2 ? 0 : turn + 1;
         if ((lane & 27) == 0) {
             atomicMax(wm, amax);
-            if (warp == 0) wmax[2 * ((n + 1) % 3) + half] = 0;
+            if (warp == 0) wmax[2 * turn + half] = 0;
         }
         __syncthreads();
         // every thread is done with the stage
-        if (tid < 128 && t + T::kStages * gridDim.x < p.n_tiles) issue(t + T::kStages * gridDim.x, s);
-        amax = *wm;
-        const uint32_t byte = scale_byte(amax);
+        if (t + T::kStages * gridDim.x < p.n_tiles) issue(t + T::kStages * gridDim.x, s);
+        if (++s == T::kStages) {
+            s = 0;
+            parity ^= 1;
+        }
+        const uint32_t byte = scale_byte(*wm);
         const float inv = inverse_scale(byte);
-        if (warp == 0 && (lane & 27) == 0 && 128 * half < cols)
-            p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + (col0 >> 7) + half] = static_cast<uint8_t>(byte);
+        if (warp == 0 && (lane & 27) == 0 && static_cast<uint32_t>(128 * half) < cols)
+            p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + 2 * tile_c + half] = static_cast<uint8_t>(byte);
         // a warp with a value that is not finite takes its own way
         const bool plain = __all_sync(0xffffffffu, finite);
+        uint8_t* out = my_out + (static_cast<int64_t>(row0) * p.cols + 256 * tile_c);
 #pragma unroll
-        for (int i = 0; i < NR; ++i) {
-            const int r = 64 * i + 4 * warp + (lane >> 3);
-            if (!col_in || r >= rows) continue;
+        for (int i = 0; i < NR; ++i, out += 64 * p.cols) {
+            if (!col_in || my_row + 64 * i >= rows) continue;
             uint32_t c[8];
             if (plain) encode32<TYPE, false>(q[i], A[i], B[i], inv, c);
             else encode32<TYPE, true>(q[i], A[i], B[i], inv, c);
-            uint8_t* out = p.codes + (static_cast<int64_t>(row0) + r) * p.cols + col0 + 32 * sub;
             if (sectors) {
                 stg256(out, c);
             } else {
@@ -359,15 +392,32 @@ __global__ void __launch_bounds__(256) gq_fp8_float_weight_kernel(const GqFp8Wei
 template <int TYPE>
 int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     using T = Fp8Tile<TYPE>;
-    auto kern = gq_fp8_weight_kernel<TYPE>;
-    static std::atomic<uint64_t> allowed{0};
-    const cudaError_t e = allow_smem(kern, T::kSmem, allowed);
+    static std::atomic<uint64_t> allowed[2]{};
+    const int64_t hd = p.head_dim / 2;
+    // boxes start on 128 bytes in shared memory: eight rows at least
+    const bool boxes = p.row_bytes % 16 == 0 && (hd == 0 || (hd >= 8 && (128 % hd == 0 || hd % 128 == 0)));
+    auto kern = boxes ? gq_fp8_weight_kernel<TYPE, true> : gq_fp8_weight_kernel<TYPE, false>;
+    const cudaError_t e = allow_smem(kern, T::kSmem, allowed[boxes]);
     if (e != cudaSuccess) return static_cast<int>(e);
+    CUtensorMap map{};
+    if (boxes) {
+        p.box_rows = static_cast<uint32_t>(hd == 0 ? 128 : std::min<int64_t>(hd, 128));
+        const EncodeTiled fn = encode_tiled();
+        if (fn == nullptr) return static_cast<int>(cudaErrorNotSupported);
+        const cuuint64_t per = hd == 0 ? 1 : 2;
+        const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.row_bytes / 4), per, static_cast<cuuint64_t>(p.rows) / per};
+        const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.row_bytes), per * static_cast<cuuint64_t>(p.row_bytes)};
+        const cuuint32_t box[3] = {T::kPitch / 4, 1, p.box_rows}, step[3] = {1, 1, 1};
+        if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t*>(p.src), dims, strides, box, step,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return static_cast<int>(cudaErrorInvalidValue);
+    }
     p.n_col_tiles = static_cast<uint32_t>((p.cols + 255) / 256);
     p.n_tiles = static_cast<uint32_t>((p.rows + 127) / 128 * p.n_col_tiles);
     fast_div_params(p.n_col_tiles, p.ncol_mul, p.ncol_shift);
     const uint32_t most = static_cast<uint32_t>(sm_count() * T::kPerSm);
-    kern<<<std::min(p.n_tiles, most), T::kThreads, T::kSmem, s>>>(p);
+    kern<<<std::min(p.n_tiles, most), T::kThreads, T::kSmem, s>>>(map, p);
     return static_cast<int>(cudaGetLastError());
 }
 template <class T>

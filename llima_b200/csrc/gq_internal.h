@@ -108,6 +108,7 @@ struct GqFp8Weight {
     uint32_t head_dim;        // > 0: llama q/k head permutation with heads of this size
     uint32_t n_col_tiles, n_tiles;   // set by the launch
     uint32_t ncol_mul, ncol_shift;   // division by n_col_tiles (fast_div_params)
+    uint32_t box_rows;
 };
 
 // Activations (rows, cols) to e4m3 codes and one E8M0 scale per 1 x 128 block.  weight set:

@@ -500,20 +500,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
 
 // ---- host side ------------------------------------------------------------------------------
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess) f = nullptr;
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return fn;
-}
-
 // (rows, k) bytes with a row stride, in boxes of box_rows x 128 bytes laid out in the
 // 128-byte swizzle
 bool tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {

@@ -151,13 +151,23 @@ def test_weight_head_permutation(fmt):
     check_weight(fmt, raw_bytes(fmt, 288, cols, 5), 288, cols, heads=3)
 
 
+@pytest.mark.parametrize("fmt", TYPES)
+@pytest.mark.parametrize("rows,cols,heads", [(300, 2048, 0), (129, 640, 0), (512, 2048, 4), (512, 2048, 8), (512, 768, 2), (640, 2048, 40),
+                                             (512, 2048, 64), (576, 2048, 3), (1024, 512, 2), (5, 2304, 0)])
+def test_weight_rows_of_whole_16_bytes_and_not(fmt, rows, cols, heads):
+    """Rows whose bytes are a multiple of 16 arrive in boxes, others one by one; heads of 128, 64,
+    256, 16, 8, 192 and 512 rows."""
+    cols = cols // FORMATS[fmt].unit_values * FORMATS[fmt].unit_values
+    check_weight(fmt, raw_bytes(fmt, rows, cols, rows + heads), rows, cols, heads)
+
+
 @pytest.mark.parametrize("fmt", [t for t in TYPES if t[0] == "Q"])
 def test_weight_of_random_bytes(fmt):
     """NaN, infinite, negative, subnormal and huge f16 constants."""
     f = FORMATS[fmt]
-    rows, cols = 260, 2 * max(128, f.unit_values)
-    raw = np.frombuffer(np.random.default_rng(9).bytes(rows * cols // f.unit_values * f.unit_bytes), np.uint8)
-    check_weight(fmt, raw, rows, cols)
+    for rows, cols in ((260, 2 * max(128, f.unit_values)), (130, 2048)):
+        raw = np.frombuffer(np.random.default_rng(9).bytes(rows * cols // f.unit_values * f.unit_bytes), np.uint8)
+        check_weight(fmt, raw, rows, cols)
 
 
 def test_weight_float_extremes():

@@ -159,6 +159,8 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
         for (int i = 0; i < 6; ++i) wmax[i] = 0;
     }
     __syncthreads();
+    let_next();
+    after_previous();
     const uint32_t all_rows = static_cast<uint32_t>(p.rows), all_cols = static_cast<uint32_t>(p.cols);
     constexpr uint32_t kColBytes = T::kChunkBytes;         // of 256 columns
     const auto issue = [&](uint32_t t, int s) {
@@ -361,6 +363,8 @@ template <class T>
 __global__ void __launch_bounds__(256) gq_fp8_float_weight_kernel(const GqFp8Weight p) {
     __shared__ uint32_t wmax[8];
     const int tid = threadIdx.x;
+    let_next();
+    after_previous();
     const int64_t row0 = static_cast<int64_t>(blockIdx.x / p.n_col_tiles) * 128;
     const int64_t col = static_cast<int64_t>(blockIdx.x % p.n_col_tiles) * 128 + 8 * (tid & 15);
     float x[8][8];
@@ -417,15 +421,13 @@ int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     p.n_tiles = static_cast<uint32_t>((p.rows + 127) / 128 * p.n_col_tiles);
     fast_div_params(p.n_col_tiles, p.ncol_mul, p.ncol_shift);
     const uint32_t most = static_cast<uint32_t>(sm_count() * T::kPerSm);
-    kern<<<std::min(p.n_tiles, most), T::kThreads, T::kSmem, s>>>(map, p);
-    return static_cast<int>(cudaGetLastError());
+    return launch_early(kern, std::min(p.n_tiles, most), T::kThreads, T::kSmem, s, 1, map, p);
 }
 template <class T>
 int launch_float_weight(GqFp8Weight& p, cudaStream_t s) {
     p.n_col_tiles = static_cast<uint32_t>((p.cols + 127) / 128);
     const int64_t tiles = (p.rows + 127) / 128 * p.n_col_tiles;
-    gq_fp8_float_weight_kernel<T><<<static_cast<unsigned>(tiles), 256, 0, s>>>(p);
-    return static_cast<int>(cudaGetLastError());
+    return launch_early(gq_fp8_float_weight_kernel<T>, static_cast<unsigned>(tiles), 256, 0, s, 1, p);
 }
 
 // ---------------------------------------------------------------------------------------
@@ -546,6 +548,8 @@ template <class T, bool GATED>
 __global__ void __launch_bounds__(256) gq_fp8_rows_kernel(const GqFp8Rows p, const uint32_t count, const uint32_t mul,
                                                           const uint32_t shift, const bool wide) {
     constexpr int E = Elem<T>::kBytes;
+    let_next();
+    after_previous();
     const uint32_t sub = threadIdx.x & 7;
     const uint32_t b = blockIdx.x * 32 + (threadIdx.x >> 3);
     const uint32_t row = fast_div(b, mul, shift);
@@ -595,6 +599,8 @@ __global__ void __launch_bounds__(512) gq_fp8_norm_kernel(const GqFp8Rows p, con
             if constexpr (RESIDUAL) r.load(p.residual + (row * p.ld_residual + c) * E, wide);
         }
     };
+    let_next();
+    after_previous();
     float4 weight[NV == 1 ? 4 : 1];
     if constexpr (NV == 1) {
         if (column(0) < p.cols)
@@ -672,6 +678,8 @@ __global__ void __launch_bounds__(512) gq_fp8_long_norm_kernel(const GqFp8Rows p
     __shared__ float wsum[16];
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
+    let_next();
+    after_previous();
     const uint8_t* from = p.x + row * p.ld_x * E;
     float2 ss = make_float2(0.0f, 0.0f);
     for (int64_t c = 16 * tid; c < p.cols; c += 16 * 512) {
@@ -722,7 +730,7 @@ __global__ void __launch_bounds__(512) gq_fp8_long_norm_kernel(const GqFp8Rows p
 }
 
 template <class T, bool RESIDUAL, int NV>
-void launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
+int launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
     auto kern = gq_fp8_norm_kernel<T, RESIDUAL, NV>;
     const int threads = static_cast<int>(((p.cols + 15) / 16 + 32 * NV - 1) / (32 * NV) * 32);
     const int sms = sm_count();
@@ -732,14 +740,14 @@ void launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, 0);
         grid = std::min<int64_t>(grid, static_cast<int64_t>(sms) * std::max(per, 1));
     }
-    kern<<<static_cast<unsigned>(grid), threads, 0, s>>>(p, wide);
+    return launch_early(kern, static_cast<unsigned>(grid), threads, 0, s, 1, p, wide);
 }
 
 template <class T, bool RESIDUAL>
-void launch_norm(const GqFp8Rows& p, bool wide, cudaStream_t s) {
-    if (p.cols <= 8192) launch_norm_rows<T, RESIDUAL, 1>(p, wide, s);
-    else if (p.cols <= 16384) launch_norm_rows<T, RESIDUAL, 2>(p, wide, s);
-    else gq_fp8_long_norm_kernel<T, RESIDUAL><<<static_cast<unsigned>(p.rows), 512, 0, s>>>(p, wide);
+int launch_norm(const GqFp8Rows& p, bool wide, cudaStream_t s) {
+    if (p.cols <= 8192) return launch_norm_rows<T, RESIDUAL, 1>(p, wide, s);
+    if (p.cols <= 16384) return launch_norm_rows<T, RESIDUAL, 2>(p, wide, s);
+    return launch_early(gq_fp8_long_norm_kernel<T, RESIDUAL>, static_cast<unsigned>(p.rows), 512, 0, s, 1, p, wide);
 }
 
 // every row starts on a 32-byte boundary
@@ -753,9 +761,7 @@ int launch_rows(GqFp8Rows p, cudaStream_t s) {
     const bool wide = rows32(p.x, p.ld_x, p.rows, E) && rows32(p.gate, p.ld_gate, p.rows, E) &&
                       rows32(p.residual, p.ld_residual, p.rows, E) && rows32(p.sum, p.ld_sum, p.rows, E);
     if (p.weight != nullptr) {
-        if (p.residual != nullptr) launch_norm<T, true>(p, wide, s);
-        else launch_norm<T, false>(p, wide, s);
-        return static_cast<int>(cudaGetLastError());
+        return p.residual != nullptr ? launch_norm<T, true>(p, wide, s) : launch_norm<T, false>(p, wide, s);
     }
     uint32_t mul, shift;
     fast_div_params(static_cast<uint32_t>(p.blocks), mul, shift);
@@ -764,14 +770,15 @@ int launch_rows(GqFp8Rows p, cudaStream_t s) {
     for (int64_t r = 0; r < all; r += run) {
         p.rows = std::min(run, all - r);
         const uint32_t count = static_cast<uint32_t>(p.rows * p.blocks);
-        if (p.gate != nullptr) gq_fp8_rows_kernel<T, true><<<(count + 31) / 32, 256, 0, s>>>(p, count, mul, shift, wide);
-        else gq_fp8_rows_kernel<T, false><<<(count + 31) / 32, 256, 0, s>>>(p, count, mul, shift, wide);
+        auto kern = p.gate != nullptr ? gq_fp8_rows_kernel<T, true> : gq_fp8_rows_kernel<T, false>;
+        const int e = launch_early(kern, (count + 31) / 32, 256, 0, s, 1, p, count, mul, shift, wide);
+        if (e != 0) return e;
         p.x += run * p.ld_x * E;
         if (p.gate != nullptr) p.gate += run * p.ld_gate * E;
         p.codes += run * p.ld_codes;
         p.scales += run * p.ld_scales;
     }
-    return static_cast<int>(cudaGetLastError());
+    return 0;
 }
 
 }  // namespace

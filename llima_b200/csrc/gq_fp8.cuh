@@ -12,7 +12,13 @@
 
 namespace gq {
 
-constexpr int kFp8Block = 128;
+// The kernels of this family are launched so that each may begin before the one ahead of it on
+// the stream has ended.  after_previous(): waits until that one has, its memory operations
+// included; every thread calls it before its first access to global memory.  let_next(): the
+// next one may begin, called once this CTA holds all that it will wait for (tensor memory).
+__device__ __forceinline__ void after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 constexpr uint32_t kInfBits = 0x7F800000u;
 
 // |x| bits where x is finite, else 0

@@ -29,6 +29,28 @@ cudaError_t allow_smem(K kern, int bytes, std::atomic<uint64_t>& done) {
     return e;
 }
 
+// A launch that may begin while the kernel before it on the stream still runs (its kernels call
+// after_previous() before they touch memory, so only their set-up overlaps); cluster > 1: in
+// clusters of that many CTAs.
+template <class... P, class... A>
+int launch_early(void (*kern)(P...), unsigned grid, int threads, int smem, cudaStream_t s, unsigned cluster, A... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(static_cast<unsigned>(threads));
+    cfg.dynamicSmemBytes = static_cast<size_t>(smem);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, P(args)...));
+}
+
 using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -14,6 +14,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include "gq_fp8.cuh"
 #include "gq_internal.h"
 #include "gq_launch.h"
 #include "gq_tcgen05.cuh"
@@ -109,6 +110,10 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     const int blocks = kb1 - kb0;
 
     if (warp == 5) tc::tmem_alloc<C::kCols>(slot);
+    if (warp == 4 && tc::elect()) {
+        tc::prefetch_map(&map_b);
+        tc::prefetch_map(&map_a);
+    }
     if (tid == 0) {
         for (int s = 0; s < C::kStages; ++s) {
             tc::init(full(s), 1);
@@ -125,13 +130,11 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     __syncthreads();
     tc::fence_after();
     const uint32_t tmem = lds_u32(slot);
+    let_next();
+    after_previous();
 
     bool ok = true;
     if (warp == 4) {
-        if (tc::elect()) {
-            tc::prefetch_map(&map_b);
-            tc::prefetch_map(&map_a);
-        }
         int issued = 0;
         for (int i = 0; i < blocks; ++i) {
             const int s = i % C::kStages, round = i / C::kStages;
@@ -148,17 +151,23 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
         if (!ok)
             for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
     } else if (warp == 5) {
+        const auto copy_group = [&](int g) {
+            const int q = g % kSfSlots;
+            if (!tc::wait(sf_full(q), (g / kSfSlots) & 1)) return false;
+            tc::fence_after();
+            if (tc::elect()) {
+                tc::copy_scales(tmem + BN + 8 * q, tc::scale_desc(sf + q * C::kSfBytes));
+                tc::copy_scales(tmem + BN + 8 * q + 4, tc::scale_desc(sf + q * C::kSfBytes + 512));
+            }
+            __syncwarp();
+            return true;
+        };
         for (int i = 0; i < blocks; ++i) {
             const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
             const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
-            if (i % 4 == 0) {
-                if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
-                tc::fence_after();
-                if (tc::elect()) {
-                    tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
-                    tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
-                }
-            }
+            if (i == 0 && !(ok = copy_group(0))) break;
+            // the next group's scales while this one's instructions run
+            if (i % 4 == 1 && i + 3 < blocks && !(ok = copy_group(g + 1))) break;
             if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
             tc::fence_after();
             if (tc::elect()) {
@@ -307,7 +316,7 @@ __device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int&
 }
 
 template <int BN, class T>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 1)
+__global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
     gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
                    const int tiles_m, const int tiles_n) {
     using C = Wide<BN>;
@@ -327,6 +336,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
     const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
 
     if (warp == 9) tc::tmem_alloc_pair<C::kCols>(slot);
+    if (warp == 8 && tc::elect()) {
+        tc::prefetch_map(&map_a);
+        tc::prefetch_map(&map_b);
+    }
     if (tid == 0) {
         for (int s = 0; s < C::kStages; ++s) {
             tc::init(full(s), 1);        // the first CTA's: both CTAs' loads
@@ -347,13 +360,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
     tc::cluster_sync();
     tc::fence_after();
     const uint32_t tmem = lds_u32(slot);
+    let_next();
+    after_previous();
 
     bool ok = true;
     if (warp == 8) {
-        if (tc::elect()) {
-            tc::prefetch_map(&map_a);
-            tc::prefetch_map(&map_b);
-        }
         int it = 0;
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
@@ -381,6 +392,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
             }
     } else if (warp == 9) {
         int it = 0, gi = 0, n = 0;
+        const auto copy_group = [&](int g) {
+            const int q = g % kSfSlots;
+            if (!tc::wait(sf_full(q), (g / kSfSlots) & 1)) return false;
+            tc::fence_after();
+            if (tc::elect()) {
+                const uint32_t from = sf + q * C::kSfBytes, to = tmem + C::kAcc * BN + C::kSfCols * q;
+                tc::copy_scales_pair(to, tc::scale_desc(from));
+#pragma unroll
+                for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(to + 4 + 4 * j, tc::scale_desc(from + 512 + 512 * j));
+            }
+            __syncwarp();
+            return true;
+        };
         for (int t = pair; rank == 0 && t < tiles && ok; t += pairs, ++n) {
             const int b = n % C::kAcc, use = n / C::kAcc;
             if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
@@ -388,16 +412,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(Wide<BN>::kThreads, 
             for (int i = 0; i < blocks; ++i, ++it) {
                 const int s = it % C::kStages, q = gi % kSfSlots;
                 const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
-                if (i % 4 == 0) {
-                    if (!(ok = tc::wait(sf_full(q), (gi / kSfSlots) & 1))) break;
-                    tc::fence_after();
-                    if (tc::elect()) {
-                        const uint32_t from = sf + q * C::kSfBytes;
-                        tc::copy_scales_pair(ta, tc::scale_desc(from));
-#pragma unroll
-                        for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
-                    }
-                }
+                if (it == 0 && !(ok = copy_group(0))) break;
+                // the next group's scales, of this tile or the next, while this one's
+                // instructions run
+                if (i % 4 == (i / 4 == groups - 1 ? 0 : 1) && (i / 4 < groups - 1 || t + pairs < tiles) && !(ok = copy_group(gi + 1)))
+                    break;
                 if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
                 tc::fence_after();
                 const bool last = i % 4 == 3 || i + 1 == blocks;
@@ -528,20 +547,8 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     const int sms = sm_count();
     while (split < 8 && tiles * split * 2 <= 2 * sms && p.kb >= 4 * split) split *= 2;
     if (tiles * split > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(tiles * split));
-    cfg.blockDim = dim3(C::kThreads);
-    cfg.dynamicSmemBytes = C::kSmem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = static_cast<unsigned>(split);
-    attr[0].val.clusterDim.y = 1;
-    attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    e = cudaLaunchKernelEx(&cfg, kern, map_b, map_a, p, split);
-    return static_cast<int>(e);
+    return launch_early(kern, static_cast<unsigned>(tiles * split), C::kThreads, C::kSmem, s, static_cast<unsigned>(split), map_b,
+                        map_a, p, split);
 }
 
 template <int BN, class T>
@@ -558,13 +565,15 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
     if (tiles_m * tiles_n * p.kb > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     const int64_t pairs = sm_count() / 2;
     const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
-    kern<<<grid, C::kThreads, C::kSmem, s>>>(map_a, map_b, p, static_cast<int>(tiles_m), static_cast<int>(tiles_n));
-    return static_cast<int>(cudaGetLastError());
+    return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, p, static_cast<int>(tiles_m),
+                        static_cast<int>(tiles_n));
 }
 
 // out = bias (or 0): a product over no columns
 template <class T>
 __global__ void gq_matmul_bias(const GqMatmul p) {
+    let_next();
+    after_previous();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < p.m * p.n;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x) {
         const int64_t m = i / p.n, n = i - m * p.n;
@@ -575,8 +584,7 @@ __global__ void gq_matmul_bias(const GqMatmul p) {
 template <class T>
 int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
-        gq_matmul_bias<T><<<1024, 256, 0, s>>>(p);
-        return static_cast<int>(cudaGetLastError());
+        return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
     if (p.m <= 16) return launch_narrow<16, T>(p, s);
     if (p.m <= 32) return launch_narrow<32, T>(p, s);

@@ -151,23 +151,18 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
         if (!ok)
             for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
     } else if (warp == 5) {
-        const auto copy_group = [&](int g) {
-            const int q = g % kSfSlots;
-            if (!tc::wait(sf_full(q), (g / kSfSlots) & 1)) return false;
-            tc::fence_after();
-            if (tc::elect()) {
-                tc::copy_scales(tmem + BN + 8 * q, tc::scale_desc(sf + q * C::kSfBytes));
-                tc::copy_scales(tmem + BN + 8 * q + 4, tc::scale_desc(sf + q * C::kSfBytes + 512));
-            }
-            __syncwarp();
-            return true;
-        };
         for (int i = 0; i < blocks; ++i) {
             const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
             const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
-            if (i == 0 && !(ok = copy_group(0))) break;
-            // the next group's scales while this one's instructions run
-            if (i % 4 == 1 && i + 3 < blocks && !(ok = copy_group(g + 1))) break;
+            if (i % 4 == 0) {
+                if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
+                tc::fence_after();
+                if (tc::elect()) {
+                    tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
+                    tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
+                }
+                __syncwarp();
+            }
             if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
             tc::fence_after();
             if (tc::elect()) {
@@ -261,6 +256,47 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
 // Warps 0-7 drain the accumulators into registers, release them and then store; warp 8 loads
 // tiles, warp 9 of the first CTA issues the matrix instructions, warp 10 stages the scales.
 
+// A tile's scales as they lie in memory: 128 rows of the tokens' and two of the weights', for all
+// of k.  They come by bulk copies, the next tile's as soon as this one's are read: the tile loads
+// keep the SM's whole read path from L2 busy (64 bytes a cycle), and a plain load queues behind
+// all of them (measured: 1000 to 3000 cycles for each group of scales).
+constexpr int kRawA = 16384, kRawB = 512;
+
+// A region of scale rows first..first + rows - 1 (those within `all`): from the 16-byte boundary
+// before it to the one after it, or to the end of the tensor, whose last bytes are `tail`.
+struct RawRegion {
+    int64_t start;      // bytes from the tensor's first
+    int skew, whole, tail;
+};
+__device__ __forceinline__ RawRegion raw_region(int64_t first, int rows, int64_t all, int64_t ld, int64_t blocks) {
+    RawRegion r{0, 0, 0, 0};
+    if (first >= all) return r;
+    const int64_t begin = first * ld, end = (min(first + rows, all) - 1) * ld + blocks, last = (all - 1) * ld + blocks;
+    r.start = begin & ~int64_t(15);
+    r.skew = static_cast<int>(begin - r.start);
+    const int64_t stop = (end + 15) & ~int64_t(15);
+    r.whole = static_cast<int>((stop <= last ? stop : end & ~int64_t(15)) - r.start);
+    r.tail = static_cast<int>(stop <= last ? 0 : end & 15);
+    return r;
+}
+// Four scale bytes at shared address a
+__device__ __forceinline__ uint32_t raw_word(uint32_t a, bool words) {
+    if (words) return lds_u32(a);
+    return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
+}
+
+// They are staged for the copy to tensor memory in batches of kBatch groups (16 blocks of 128
+// columns), two batches in turn: the fence and the remote arrival that a batch ends with take
+// longer than the instructions of one group of a narrow tile.
+constexpr int kBatch = 4;
+
+// Four scale bytes at `off` of a region whose first `whole` bytes are in shared memory at `raw`
+__device__ __forceinline__ uint32_t raw_word(uint32_t raw, int off, int whole, const uint8_t* row, int64_t kb, int64_t blocks) {
+    if (off + 4 > whole) return scale_word(row, kb, blocks);
+    const uint32_t a = raw + off;
+    return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
+}
+
 template <int BN>
 struct Wide {
     static constexpr int kThreads = 352;
@@ -270,11 +306,12 @@ struct Wide {
     static constexpr int kSfBytes = 512 + 512 * (BN / 128);
     static constexpr int kSfCols = 4 + 4 * (BN / 128);
     static constexpr int kAcc = BN == 256 ? 1 : 2;             // accumulators in tensor memory
-    static constexpr int kBars = 2 * kStages + 2 * kSfSlots + 2 * kAcc;
+    static constexpr int kSlots = 2 * kBatch;
+    static constexpr int kBars = 2 * kStages + 2 * 2 + 2 * kAcc + 1;
     static constexpr int kCols = 512;
     static constexpr int kSmem = 227 * 1024;                   // all of an SM's, as all of its tensor memory
-    static_assert(1024 + kStages * kStageBytes + kSfSlots * kSfBytes + 8 * kBars + 16 <= kSmem, "shared memory");
-    static_assert(kAcc * BN + kSfSlots * kSfCols <= kCols, "tensor memory");
+    static_assert(1024 + kStages * kStageBytes + kSlots * kSfBytes + kRawA + kRawB + 8 * kBars + 16 <= kSmem, "shared memory");
+    static_assert(kAcc * BN + kSlots * kSfCols <= kCols, "tensor memory");
 };
 
 // 32 bytes to one row of the output: the values of columns n.. (T of 2 or 4 bytes)
@@ -318,23 +355,24 @@ __device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int&
 template <int BN, class T>
 __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
     gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
-                   const int tiles_m, const int tiles_n) {
+                   const int tiles_m, const int tiles_n, const bool use_raw) {
     using C = Wide<BN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sf = base + C::kStages * C::kStageBytes, bars = sf + kSfSlots * C::kSfBytes, slot = bars + 8 * C::kBars;
+    const uint32_t sf = base + C::kStages * C::kStageBytes, raw_a = sf + C::kSlots * C::kSfBytes, raw_b = raw_a + kRawA;
+    const uint32_t bars = raw_b + kRawB, slot = bars + 8 * C::kBars;
     const auto full = [&](int s) { return bars + 8 * s; };
     const auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
     const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
-    const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + kSfSlots + s); };
-    const auto acc_full = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + s); };
-    const auto acc_empty = [&](int s) { return bars + 8 * (2 * C::kStages + 2 * kSfSlots + C::kAcc + s); };
+    const auto sf_empty = [&](int s) { return bars + 8 * (2 * C::kStages + 2 + s); };
+    const uint32_t raw_full = bars + 8 * (C::kBars - 1);
+    const auto acc_full = [&](int s) { return bars + 8 * (2 * C::kStages + 4 + s); };
+    const auto acc_empty = [&](int s) { return bars + 8 * (2 * C::kStages + 4 + C::kAcc + s); };
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform for the compiler
     const uint32_t rank = tc::cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
     const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
-
     if (warp == 9) tc::tmem_alloc_pair<C::kCols>(slot);
     if (warp == 8 && tc::elect()) {
         tc::prefetch_map(&map_a);
@@ -345,7 +383,7 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
             tc::init(full(s), 1);        // the first CTA's: both CTAs' loads
             tc::init(empty(s), 1);
         }
-        for (int s = 0; s < kSfSlots; ++s) {
+        for (int s = 0; s < 2; ++s) {
             tc::init(sf_full(s), 2);
             tc::init(sf_empty(s), 1);
         }
@@ -353,6 +391,7 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
             tc::init(acc_full(s), 1);
             tc::init(acc_empty(s), 16);  // the first CTA's: eight warps of both CTAs
         }
+        tc::init(raw_full, 1);
         mbar_init_fence();
     }
     tc::fence_before();
@@ -391,35 +430,30 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
             for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
             }
     } else if (warp == 9) {
-        int it = 0, gi = 0, n = 0;
-        const auto copy_group = [&](int g) {
-            const int q = g % kSfSlots;
-            if (!tc::wait(sf_full(q), (g / kSfSlots) & 1)) return false;
-            tc::fence_after();
-            if (tc::elect()) {
-                const uint32_t from = sf + q * C::kSfBytes, to = tmem + C::kAcc * BN + C::kSfCols * q;
-                tc::copy_scales_pair(to, tc::scale_desc(from));
-#pragma unroll
-                for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(to + 4 + 4 * j, tc::scale_desc(from + 512 + 512 * j));
-            }
-            __syncwarp();
-            return true;
-        };
+        int it = 0, bi = 0, n = 0;     // blocks, batches and tiles so far
         for (int t = pair; rank == 0 && t < tiles && ok; t += pairs, ++n) {
             const int b = n % C::kAcc, use = n / C::kAcc;
             if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
             tc::fence_after();
             for (int i = 0; i < blocks; ++i, ++it) {
-                const int s = it % C::kStages, q = gi % kSfSlots;
+                const int s = it % C::kStages, q = (bi & 1) * kBatch + i / 4 % kBatch;
                 const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
-                if (it == 0 && !(ok = copy_group(0))) break;
-                // the next group's scales, of this tile or the next, while this one's
-                // instructions run
-                if (i % 4 == (i / 4 == groups - 1 ? 0 : 1) && (i / 4 < groups - 1 || t + pairs < tiles) && !(ok = copy_group(gi + 1)))
-                    break;
+                if (i % (4 * kBatch) == 0) {
+                    if (!(ok = tc::wait(sf_full(bi & 1), (bi >> 1) & 1))) break;
+                    tc::fence_after();
+                }
+                if (i % 4 == 0) {
+                    if (tc::elect()) {
+                        const uint32_t from = sf + q * C::kSfBytes;
+                        tc::copy_scales_pair(ta, tc::scale_desc(from));
+#pragma unroll
+                        for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
+                    }
+                    __syncwarp();
+                }
                 if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
                 tc::fence_after();
-                const bool last = i % 4 == 3 || i + 1 == blocks;
+                const bool last = i % (4 * kBatch) == 4 * kBatch - 1 || i + 1 == blocks;
                 if (tc::elect()) {
                     const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
                     const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
@@ -427,43 +461,96 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
 #pragma unroll
                     for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
                     tc::commit_pair(empty(s));
-                    if (last) tc::commit_pair(sf_empty(q));
+                    if (last) tc::commit_pair(sf_empty(bi & 1));
                 }
                 __syncwarp();
-                if (last) ++gi;
+                if (last) ++bi;
             }
             if (tc::elect()) tc::commit_pair(acc_full(b));
             __syncwarp();
         }
     } else if (warp == 10) {
-        int gi = 0;
+        constexpr int kB = BN / 128;
+        int bi = 0;
+        const int64_t nbs = (p.n + 127) >> 7;
+        RawRegion ra{0, 0, 0, 0}, rb{0, 0, 0, 0};
+        const bool words = ((p.ld_a_scales | p.ld_b_scales) & 3) == 0;
+        int asked = 0, read = 0;      // requests made, and waited for
+        const auto request = [&](int t) {
+            ++asked;
+            int tm, tn;
+            tile_place(t, tiles_m, tiles_n, tm, tn);
+            ra = raw_region(static_cast<int64_t>(tm) * 256 + 128 * rank, 128, p.m, p.ld_a_scales, p.kb);
+            rb = raw_region(static_cast<int64_t>(tn) * kB, kB, nbs, p.ld_b_scales, p.kb);
+            if (tc::elect()) {
+                tc::arrive_expect(raw_full, static_cast<uint32_t>(ra.whole + rb.whole));
+                if (ra.whole > 0) tc::bulk(raw_a, p.a_scales + ra.start, ra.whole, raw_full);
+                if (rb.whole > 0) tc::bulk(raw_b, p.b_scales + rb.start, rb.whole, raw_full);
+            }
+            __syncwarp();
+        };
+        // the very first batch is read as it lies in global memory, ahead of the first tile loads
+        if (use_raw && pair < tiles && groups > kBatch) request(pair);
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
             tile_place(t, tiles_m, tiles_n, tm, tn);
-            const int64_t m0 = static_cast<int64_t>(tm) * 256 + 128 * rank;
-            const int64_t nb0 = static_cast<int64_t>(tn) * (BN / 128), nbs = (p.n + 127) >> 7;
-            for (int g = 0; g < groups; ++g, ++gi) {
-                const int q = gi % kSfSlots, round = gi / kSfSlots;
-                uint32_t x[4], w[BN / 128];
+            const int64_t m0 = static_cast<int64_t>(tm) * 256 + 128 * rank, nb0 = static_cast<int64_t>(tn) * kB;
+            uint32_t from_a[4] = {0, 0, 0, 0}, from_b[kB] = {};
+            bool raw = false;
+            for (int g0 = 0; g0 < groups; g0 += kBatch, ++bi) {
+                if (use_raw && !raw && bi > 0) {
+                    if (!(ok = tc::wait(raw_full, read & 1))) break;
+                    ++read;
+                    raw = true;
+                    if (lane < ra.tail) sts(raw_a + ra.whole + lane, p.a_scales[ra.start + ra.whole + lane]);
+                    if (lane < rb.tail) sts(raw_b + rb.whole + lane, p.b_scales[rb.start + rb.whole + lane]);
+                    __syncwarp();
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int64_t m = m0 + 32 * j + lane;
-                    x[j] = m < p.m ? scale_word(p.a_scales + m * p.ld_a_scales, 4 * g, blocks) : 0x7F7F7F7Fu;
+                    for (int j = 0; j < 4; ++j) from_a[j] = raw_a + ra.skew + static_cast<uint32_t>((32 * j + lane) * p.ld_a_scales);
+#pragma unroll
+                    for (int j = 0; j < kB; ++j) from_b[j] = raw_b + rb.skew + static_cast<uint32_t>(j * p.ld_b_scales);
                 }
+                uint32_t x[kBatch][4], w[kBatch][kB];
 #pragma unroll
-                for (int j = 0; j < BN / 128; ++j)
-                    w[j] = nb0 + j < nbs ? scale_word(p.b_scales + (nb0 + j) * p.ld_b_scales, 4 * g, blocks) : 0x7F7F7F7Fu;
-                if (round > 0 && !(ok = tc::wait(sf_empty(q), (round - 1) & 1))) break;
-                const uint32_t to = sf + q * C::kSfBytes + 16 * lane;
-                sts(to, make_uint4(x[0], x[1], x[2], x[3]));
+                for (int u = 0; u < kBatch; ++u) {
+                    const int kb = 4 * (g0 + u);
+                    if (g0 + u >= groups) continue;
 #pragma unroll
-                for (int j = 0; j < BN / 128; ++j) sts(to + 512 + 512 * j, make_uint4(w[j], w[j], w[j], w[j]));
+                    for (int j = 0; j < 4; ++j) {
+                        const int64_t m = m0 + 32 * j + lane;
+                        x[u][j] = m >= p.m ? 0x7F7F7F7Fu
+                                  : raw    ? raw_word(from_a[j] + kb, words)
+                                           : scale_word(p.a_scales + m * p.ld_a_scales, kb, blocks);
+                    }
+#pragma unroll
+                    for (int j = 0; j < kB; ++j)
+                        w[u][j] = nb0 + j >= nbs ? 0x7F7F7F7Fu
+                                  : raw          ? raw_word(from_b[j] + kb, words)
+                                                 : scale_word(p.b_scales + (nb0 + j) * p.ld_b_scales, kb, blocks);
+                }
+                // this tile's are read: the next one's may overwrite them
+                if (use_raw && g0 + kBatch >= groups && t + pairs < tiles) {
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    request(t + pairs);
+                }
+                if (bi > 1 && !(ok = tc::wait(sf_empty(bi & 1), ((bi >> 1) - 1) & 1))) break;
+#pragma unroll
+                for (int u = 0; u < kBatch; ++u) {
+                    if (g0 + u >= groups) continue;
+                    const uint32_t to = sf + ((bi & 1) * kBatch + u) * C::kSfBytes + 16 * lane;
+                    sts(to, make_uint4(x[u][0], x[u][1], x[u][2], x[u][3]));
+#pragma unroll
+                    for (int j = 0; j < kB; ++j) sts(to + 512 + 512 * j, make_uint4(w[u][j], w[u][j], w[u][j], w[u][j]));
+                }
                 tc::fence_async_shared();
                 __syncwarp();
-                if (lane == 0) tc::arrive_remote(tc::map_shared(sf_full(q), 0));
+                if (lane == 0) tc::arrive_remote(tc::map_shared(sf_full(bi & 1), 0));
             }
         }
-        for (int i = max(0, gi - kSfSlots); ok && i < gi; ++i) ok = tc::wait(sf_empty(i % kSfSlots), (i / kSfSlots) & 1);
+        // a request that nothing waited for, after a wait that gave up
+        if (!ok && asked > read) tc::wait(raw_full, read & 1);
+        for (int i = max(0, bi - 2); ok && i < bi; ++i) ok = tc::wait(sf_empty(i & 1), (i >> 1) & 1);
     } else {
         constexpr int kPart = BN / 2;                       // columns per warp
         int n = 0;
@@ -563,10 +650,12 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles_m = (p.m + 255) / 256, tiles_n = (p.n + BN - 1) / BN;
     if (tiles_m * tiles_n * p.kb > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
+    const bool use_raw = (reinterpret_cast<uintptr_t>(p.a_scales) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.b_scales) & 15) == 0 &&
+                         128 * p.ld_a_scales <= kRawA && BN / 128 * p.ld_b_scales + 32 <= kRawB;
     const int64_t pairs = sm_count() / 2;
     const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
     return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, p, static_cast<int>(tiles_m),
-                        static_cast<int>(tiles_n));
+                        static_cast<int>(tiles_n), use_raw);
 }
 
 // out = bias (or 0): a product over no columns

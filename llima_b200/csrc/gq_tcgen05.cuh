@@ -42,6 +42,13 @@ __device__ __forceinline__ void load_box(uint32_t dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// `bytes` (a multiple of 16) from a 16-byte-aligned address
+__device__ __forceinline__ void bulk(uint32_t dst, const void* src, int bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cta.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src),
+                 "r"(bytes), "r"(bar)
+                 : "memory");
+}
+
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }

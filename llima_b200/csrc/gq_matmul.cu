@@ -14,6 +14,8 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <algorithm>
+
 #include "gq_fp8.cuh"
 #include "gq_internal.h"
 #include "gq_launch.h"
@@ -619,6 +621,14 @@ bool tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64
               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How k is split: until about two CTAs per SM, with at least two 128-column blocks for each.
+int narrow_split(const GqMatmul& p, int bn, int sms) {
+    const int64_t tiles = (p.m + bn - 1) / bn * ((p.n + 127) / 128);
+    int split = 1;
+    while (split < 8 && tiles * split <= sms && p.kb >= 4 * split) split *= 2;
+    return split;
+}
+
 template <int BN, class T>
 int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     using C = Narrow<BN>;
@@ -630,9 +640,7 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles = (p.m + BN - 1) / BN * ((p.n + 127) / 128);
-    int split = 1;
-    const int sms = sm_count();
-    while (split < 8 && tiles * split * 2 <= 2 * sms && p.kb >= 4 * split) split *= 2;
+    const int split = narrow_split(p, BN, sm_count());
     if (tiles * split > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     return launch_early(kern, static_cast<unsigned>(tiles * split), C::kThreads, C::kSmem, s, static_cast<unsigned>(split), map_b,
                         map_a, p, split);
@@ -658,6 +666,41 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
                         static_cast<int>(tiles_n), use_raw);
 }
 
+// Which kernel and tile: the least estimated time (us).  A narrow tile costs what its operands
+// take through an SM's read path (133 KB a us), the busiest SM counts, and no less than reading
+// the operands from HBM (6.3 MB a us); set-up and the sums' way out grow with the tile.  A wide
+// one costs its matrix instructions (0.287 us per 256 x 256 x 128 on a pair, 0.19 per 256 x 128 x
+// 128, where shared memory bounds it) and a drain, in rounds over the pairs.  Measured against
+// it (us, k = 4096 unless said; the best and the runner-up): 64 x 28672 narrow 64 23.1, narrow 128
+// 24.1; 96 x 28672 narrow 128 25.4, wide 256 30.7; 160 x 28672 wide 256 31.9, wide 128 34.5; 128 x
+// 4096 narrow 64 9.0, narrow 128 11.6; 512 x 4096 wide 128 13.4, narrow 64 14.3; 768 x 4096 wide 256
+// 19.0, wide 128 19.9; 160 x 4096, k = 14336 narrow 128 19.9, narrow 64 23.6.
+// Returns the narrow tile's tokens, or twice the wide tile's output channels.
+int choose(const GqMatmul& p) {
+    const int sms = sm_count();
+    const double hbm = static_cast<double>(p.m + p.n) * static_cast<double>(p.k) / 6.3e6;
+    int best = 16;
+    double least = 1e30;
+    const auto take = [&](int what, double us) {
+        if (us < least) {
+            least = us;
+            best = what;
+        }
+    };
+    for (int bn : {16, 32, 64, 128}) {
+        const int split = narrow_split(p, bn, sms);
+        const int64_t ctas = (p.m + bn - 1) / bn * ((p.n + 127) / 128) * split;
+        const double bytes = static_cast<double>((ctas + sms - 1) / sms) * static_cast<double>((p.kb + split - 1) / split) * (128 + bn) * 128;
+        take(bn, 3.0 + 0.032 * bn + (split > 1 ? 1.0 : 0.0) + std::max(bytes / 133e3, hbm));
+    }
+    for (int bn : {128, 256}) {
+        const int64_t tiles = (p.m + 255) / 256 * ((p.n + bn - 1) / bn), pairs = sms / 2;
+        const double each = bn == 128 ? 0.19 * static_cast<double>(p.kb) + 1.7 : 0.287 * static_cast<double>(p.kb) + 2.8;
+        take(2 * bn, 5.0 + std::max(static_cast<double>((tiles + pairs - 1) / pairs) * each, hbm));
+    }
+    return best;
+}
+
 // out = bias (or 0): a product over no columns
 template <class T>
 __global__ void gq_matmul_bias(const GqMatmul p) {
@@ -675,13 +718,14 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
         return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
-    if (p.m <= 16) return launch_narrow<16, T>(p, s);
-    if (p.m <= 32) return launch_narrow<32, T>(p, s);
-    if (p.m <= 64) return launch_narrow<64, T>(p, s);
-    if (p.m <= 256) return launch_narrow<128, T>(p, s);
-    const int64_t wide = (p.m + 255) / 256 * ((p.n + 255) / 256);
-    if (2 * wide >= sm_count()) return launch_wide<256, T>(p, s);
-    return launch_wide<128, T>(p, s);
+    switch (choose(p)) {
+        case 16: return launch_narrow<16, T>(p, s);
+        case 32: return launch_narrow<32, T>(p, s);
+        case 64: return launch_narrow<64, T>(p, s);
+        case 128: return launch_narrow<128, T>(p, s);
+        case 2 * 128: return launch_wide<128, T>(p, s);
+        default: return launch_wide<256, T>(p, s);
+    }
 }
 
 }  // namespace

@@ -68,7 +68,12 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int64_t kb, i
 constexpr int kTileK = 128;
 constexpr int kSfSlots = 4;      // groups of four 128-column blocks whose scales are staged
 
-template <int BN>
+// The matrix instructions truncate as they add, so a sum's error grows with its length (1.7e-6 of
+// the result's norm over 112 blocks).  Where the output keeps f32, a sum is taken in pieces of
+// about kPiece blocks that are added in f32 with rounding; 16-bit outputs lose nothing by it.
+constexpr int kPiece = 32;
+
+template <int BN, class T>
 struct Narrow {
     static constexpr int kThreads = 192;
     static constexpr int kStageBytes = 128 * kTileK + BN * kTileK;
@@ -77,7 +82,9 @@ struct Narrow {
     static constexpr int kBars = 2 * kStages + 2 * kSfSlots + 1;
     static constexpr int kRing = kStages * kStageBytes;            // reused for the f32 sums
     static constexpr int kUsed = 1024 + kRing + kSfSlots * kSfBytes + 8 * kBars + 16;
-    static constexpr int kCols = BN + 8 * kSfSlots <= 64 ? 64 : BN + 8 * kSfSlots <= 128 ? 128 : 256;
+    static constexpr int kPieces = sizeof(T) < 4 || BN == 128 ? 1 : BN == 16 ? 4 : 3;      // accumulators
+    static constexpr int kNeed = kPieces * BN + 8 * kSfSlots;
+    static constexpr int kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
     // CTAs that share an SM must find room in its 512 columns of tensor memory together, so
     // that none waits for another's (in a cluster that could be a circle): shared memory is
     // taken in the same proportion, 228 KB for 512 columns.
@@ -88,10 +95,10 @@ struct Narrow {
 };
 
 template <int BN, class T>
-__global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const __grid_constant__ CUtensorMap map_b,
+__global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(const __grid_constant__ CUtensorMap map_b,
                                                                          const __grid_constant__ CUtensorMap map_a,
                                                                          const GqMatmul p, const int split) {
-    using C = Narrow<BN>;
+    using C = Narrow<BN, T>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
     uint8_t* const smem = smem_raw + (base - smem_u32addr(smem_raw));
@@ -110,6 +117,7 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     const int64_t m0 = tile % m_tiles * BN, n0 = tile / m_tiles * 128;
     const int kb0 = static_cast<int>(p.kb * rank / split), kb1 = static_cast<int>(p.kb * (rank + 1) / split);
     const int blocks = kb1 - kb0;
+    const int pieces = min(C::kPieces, (blocks + kPiece - 1) / kPiece), piece = (blocks + pieces - 1) / pieces;
 
     if (warp == 5) tc::tmem_alloc<C::kCols>(slot);
     if (warp == 4 && tc::elect()) {
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
     } else if (warp == 5) {
         for (int i = 0; i < blocks; ++i) {
             const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
-            const uint32_t ta = tmem + BN + 8 * q, tb = ta + 4;
+            const uint32_t ta = tmem + C::kPieces * BN + 8 * q, tb = ta + 4;
             if (i % 4 == 0) {
                 if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
                 tc::fence_after();
@@ -172,7 +180,8 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
                 const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
                 const uint32_t idesc = tc::instruction<128, BN>(i % 4);
 #pragma unroll
-                for (int k = 0; k < 4; ++k) tc::mma(tmem, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
+                for (int k = 0; k < 4; ++k)
+                    tc::mma(tmem + BN * (i / piece), da + 2 * k, db + 2 * k, idesc, ta, tb, i % piece > 0 || k > 0);
                 tc::commit(empty(s));
                 if (i % 4 == 3 || i + 1 == blocks) tc::commit(sf_empty(q));
             }
@@ -211,8 +220,15 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
             uint32_t v[16];
             tc::tmem_load16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + c, v);
             tc::tmem_wait();
+            for (int k = 1; k < pieces; ++k) {
+                uint32_t more[16];
+                tc::tmem_load16(tmem + (static_cast<uint32_t>(32 * warp) << 16) + BN * k + c, more);
+                tc::tmem_wait();
 #pragma unroll
-            for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + 32 * warp + lane] = blocks > 0 ? __uint_as_float(v[j]) : 0.0f;
+                for (int j = 0; j < 16; ++j) v[j] = __float_as_uint(__fadd_rn(__uint_as_float(v[j]), __uint_as_float(more[j])));
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + 32 * warp + lane] = __uint_as_float(v[j]);
         }
         tc::fence_before();
     }
@@ -255,8 +271,9 @@ __global__ void __launch_bounds__(Narrow<BN>::kThreads) gq_matmul_narrow(const _
 // gq_matmul_wide: a persistent grid of CTA pairs (cta_group::2), each pair on a tile of 256
 // tokens (128 per CTA) x BN output channels; every CTA loads its own tokens' rows and half of
 // the weights' rows, so a pair reads as much from L2 as one CTA with a tile half as wide.
-// Warps 0-7 drain the accumulators into registers, release them and then store; warp 8 loads
-// tiles, warp 9 of the first CTA issues the matrix instructions, warp 10 stages the scales.
+// The first 8 warps (16 for f32 outputs) drain the accumulators into registers, release them and
+// then store; of the last three, one loads tiles, one (of the first CTA) issues the matrix
+// instructions and one stages the scales.
 
 // A tile's scales as they lie in memory: 128 rows of the tokens' and two of the weights', for all
 // of k.  They come by bulk copies, the next tile's as soon as this one's are read: the tile loads
@@ -299,9 +316,12 @@ __device__ __forceinline__ uint32_t raw_word(uint32_t raw, int off, int whole, c
     return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
 }
 
-template <int BN>
+template <int BN, class T>
 struct Wide {
-    static constexpr int kThreads = 352;
+    // warps that take the accumulators out: f32 outputs need room for a piece beside the sum
+    static constexpr int kOut = sizeof(T) == 4 ? 16 : 8;
+    static constexpr int kPieceBlocks = sizeof(T) == 4 ? kPiece : INT32_MAX;
+    static constexpr int kThreads = 32 * (kOut + 3);
     static constexpr int kHalf = BN / 2;                       // weight rows per CTA
     static constexpr int kStageBytes = 128 * kTileK + kHalf * kTileK;
     static constexpr int kStages = BN == 256 ? 6 : 8;
@@ -355,10 +375,10 @@ __device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int&
 }
 
 template <int BN, class T>
-__global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
+__global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
     gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
                    const int tiles_m, const int tiles_n, const bool use_raw) {
-    using C = Wide<BN>;
+    using C = Wide<BN, T>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t sf = base + C::kStages * C::kStageBytes, raw_a = sf + C::kSlots * C::kSfBytes, raw_b = raw_a + kRawA;
@@ -375,8 +395,8 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
     const uint32_t rank = tc::cluster_rank();
     const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
     const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
-    if (warp == 9) tc::tmem_alloc_pair<C::kCols>(slot);
-    if (warp == 8 && tc::elect()) {
+    if (warp == C::kOut + 1) tc::tmem_alloc_pair<C::kCols>(slot);
+    if (warp == C::kOut && tc::elect()) {
         tc::prefetch_map(&map_a);
         tc::prefetch_map(&map_b);
     }
@@ -391,7 +411,7 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
         }
         for (int s = 0; s < C::kAcc; ++s) {
             tc::init(acc_full(s), 1);
-            tc::init(acc_empty(s), 16);  // the first CTA's: eight warps of both CTAs
+            tc::init(acc_empty(s), 2 * C::kOut);  // the first CTA's: both CTAs' warps
         }
         tc::init(raw_full, 1);
         mbar_init_fence();
@@ -405,7 +425,7 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
     after_previous();
 
     bool ok = true;
-    if (warp == 8) {
+    if (warp == C::kOut) {
         int it = 0;
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
@@ -431,13 +451,15 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
         if (!ok)
             for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
             }
-    } else if (warp == 9) {
-        int it = 0, bi = 0, n = 0;     // blocks, batches and tiles so far
-        for (int t = pair; rank == 0 && t < tiles && ok; t += pairs, ++n) {
-            const int b = n % C::kAcc, use = n / C::kAcc;
-            if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
-            tc::fence_after();
-            for (int i = 0; i < blocks; ++i, ++it) {
+    } else if (warp == C::kOut + 1) {
+        int it = 0, bi = 0, n = 0;     // blocks, batches and pieces so far
+        for (int t = pair; rank == 0 && t < tiles && ok; t += pairs) {
+            for (int i = 0, j = 0; i < blocks; ++i, ++it) {      // j: the block's number in its piece
+                const int b = n % C::kAcc, use = n / C::kAcc;
+                if (j == 0) {
+                    if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
+                    tc::fence_after();
+                }
                 const int s = it % C::kStages, q = (bi & 1) * kBatch + i / 4 % kBatch;
                 const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
                 if (i % (4 * kBatch) == 0) {
@@ -461,17 +483,24 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
                     const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
                     const uint32_t idesc = tc::instruction<256, BN>(i % 4);
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, i > 0 || k > 0);
+                    for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, j > 0 || k > 0);
                     tc::commit_pair(empty(s));
                     if (last) tc::commit_pair(sf_empty(bi & 1));
                 }
                 __syncwarp();
                 if (last) ++bi;
+                if (++j == C::kPieceBlocks || i + 1 == blocks) {
+                    if (tc::elect()) tc::commit_pair(acc_full(b));
+                    __syncwarp();
+                    j = 0;
+                    ++n;
+                }
             }
-            if (tc::elect()) tc::commit_pair(acc_full(b));
+            // after a wait that gave up: those who wait for this piece end sooner
+            if (!ok && tc::elect()) tc::commit_pair(acc_full(n % C::kAcc));
             __syncwarp();
         }
-    } else if (warp == 10) {
+    } else if (warp == C::kOut + 2) {
         constexpr int kB = BN / 128;
         int bi = 0;
         const int64_t nbs = (p.n + 127) >> 7;
@@ -554,26 +583,40 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
         if (!ok && asked > read) tc::wait(raw_full, read & 1);
         for (int i = max(0, bi - 2); ok && i < bi; ++i) ok = tc::wait(sf_empty(i & 1), (i >> 1) & 1);
     } else {
-        constexpr int kPart = BN / 2;                       // columns per warp
+        constexpr int kPart = BN / (C::kOut / 4);           // columns per warp
         int n = 0;
-        for (int t = pair; t < tiles && ok; t += pairs, ++n) {
+        for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
             tile_place(t, tiles_m, tiles_n, tm, tn);
-            const int b = n % C::kAcc, use = n / C::kAcc;
-            if (!(ok = tc::wait(acc_full(b), use & 1))) break;
-            __syncwarp();
-            tc::fence_after();
             const int64_t m = static_cast<int64_t>(tm) * 256 + 128 * rank + 32 * (warp & 3) + lane;
             const int64_t n0 = static_cast<int64_t>(tn) * BN + kPart * (warp >> 2);
-            const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + BN * b + kPart * (warp >> 2);
-            // the accumulators are free for the next tile once they are in registers
             uint32_t v[kPart];
+            for (int i = 0; i < blocks; i += min(C::kPieceBlocks, blocks), ++n) {
+                const int b = n % C::kAcc, use = n / C::kAcc;
+                if (!(ok = tc::wait(acc_full(b), use & 1))) break;
+                __syncwarp();
+                tc::fence_after();
+                const uint32_t from = tmem + (static_cast<uint32_t>(32 * (warp & 3)) << 16) + BN * b + kPart * (warp >> 2);
+                if (sizeof(T) < 4 || i == 0) {
 #pragma unroll
-            for (int c = 0; c < kPart; c += 32) tc::tmem_load32(from + c, v + c);
-            tc::tmem_wait();
-            tc::fence_before();
-            __syncwarp();
-            if (lane == 0) tc::arrive_remote(tc::map_shared(acc_empty(b), 0));
+                    for (int c = 0; c < kPart; c += 32) tc::tmem_load32(from + c, v + c);
+                    tc::tmem_wait();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < kPart; c += 16) {
+                        uint32_t more[16];
+                        tc::tmem_load16(from + c, more);
+                        tc::tmem_wait();
+#pragma unroll
+                        for (int k = 0; k < 16; ++k) v[c + k] = __float_as_uint(__fadd_rn(__uint_as_float(v[c + k]), __uint_as_float(more[k])));
+                    }
+                }
+                // the accumulators are free for the next piece once they are in registers
+                tc::fence_before();
+                __syncwarp();
+                if (lane == 0) tc::arrive_remote(tc::map_shared(acc_empty(b), 0));
+            }
+            if (!ok) break;
             if (p.bias != nullptr) {
 #pragma unroll
                 for (int i = 0; i < kPart; ++i)
@@ -600,7 +643,7 @@ __global__ void __launch_bounds__(Wide<BN>::kThreads, 1)
     tc::fence_before();
     __syncthreads();
     tc::cluster_sync();
-    if (warp == 9) {
+    if (warp == C::kOut + 1) {
         tc::fence_after();
         tc::tmem_free_pair<C::kCols>(tmem);
     }
@@ -631,7 +674,7 @@ int narrow_split(const GqMatmul& p, int bn, int sms) {
 
 template <int BN, class T>
 int launch_narrow(const GqMatmul& p, cudaStream_t s) {
-    using C = Narrow<BN>;
+    using C = Narrow<BN, T>;
     auto kern = gq_matmul_narrow<BN, T>;
     CUtensorMap map_b, map_a;
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, 128) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, BN))
@@ -648,7 +691,7 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
 
 template <int BN, class T>
 int launch_wide(const GqMatmul& p, cudaStream_t s) {
-    using C = Wide<BN>;
+    using C = Wide<BN, T>;
     auto kern = gq_matmul_wide<BN, T>;
     CUtensorMap map_b, map_a;
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
@@ -676,7 +719,7 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
 // 4096 narrow 64 9.0, narrow 128 11.6; 512 x 4096 wide 128 13.4, narrow 64 14.3; 768 x 4096 wide 256
 // 19.0, wide 128 19.9; 160 x 4096, k = 14336 narrow 128 19.9, narrow 64 23.6.
 // Returns the narrow tile's tokens, or twice the wide tile's output channels.
-int choose(const GqMatmul& p) {
+int choose(const GqMatmul& p, bool f32) {
     const int sms = sm_count();
     const double hbm = static_cast<double>(p.m + p.n) * static_cast<double>(p.k) / 6.3e6;
     int best = 16;
@@ -689,6 +732,7 @@ int choose(const GqMatmul& p) {
     };
     for (int bn : {16, 32, 64, 128}) {
         const int split = narrow_split(p, bn, sms);
+        if (f32 && bn == 128 && p.kb > 3 * kPiece / 2 * split) continue;      // a sum in one piece (see kPiece)
         const int64_t ctas = (p.m + bn - 1) / bn * ((p.n + 127) / 128) * split;
         const double bytes = static_cast<double>((ctas + sms - 1) / sms) * static_cast<double>((p.kb + split - 1) / split) * (128 + bn) * 128;
         take(bn, 3.0 + 0.032 * bn + (split > 1 ? 1.0 : 0.0) + std::max(bytes / 133e3, hbm));
@@ -718,7 +762,7 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
         return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
-    switch (choose(p)) {
+    switch (choose(p, sizeof(T) == 4)) {
         case 16: return launch_narrow<16, T>(p, s);
         case 32: return launch_narrow<32, T>(p, s);
         case 64: return launch_narrow<64, T>(p, s);

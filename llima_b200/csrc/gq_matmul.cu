@@ -238,9 +238,25 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
     else __syncthreads();
 
     T* const out = reinterpret_cast<T*>(p.out);
+    const bool fours = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
     const int rows = static_cast<int>(min(static_cast<int64_t>(BN), p.m - m0));
     for (int u = static_cast<int>(rank) * C::kThreads + tid; u < 32 * rows; u += C::kThreads * split) {
         const int r = u >> 5, c = 4 * (u & 31);
+        if (!fours) {
+            // rows off the boundaries of four values: neighbouring lanes on neighbouring values
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int n = (u & 31) + 32 * i;
+                if (n0 + n >= p.n) continue;
+                const uint32_t at = base + (r * 128 + n) * 4;
+                float v = 0.0f;
+                for (int s = 0; s < split; ++s)
+                    v = __fadd_rn(v, split > 1 ? tc::load_cluster1(tc::map_shared(at, s)) : *reinterpret_cast<const float*>(smem + (r * 128 + n) * 4));
+                if (p.bias != nullptr) v = __fadd_rn(v, p.bias[n0 + n]);
+                out[(m0 + r) * p.ld_out + n0 + n] = out_cast<T>(v);
+            }
+            continue;
+        }
         if (n0 + c >= p.n) continue;
         float v[4] = {0, 0, 0, 0};
         const uint32_t at = base + (r * 128 + c) * 4;
@@ -316,7 +332,10 @@ __device__ __forceinline__ uint32_t raw_word(uint32_t raw, int off, int whole, c
     return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
 }
 
-template <int BN, class T>
+// STAGED: outputs whose rows do not start on 32 bytes go out through shared memory, a row's values
+// side by side from neighbouring lanes; a stage of the ring (two for f32 in narrow tiles) makes
+// room.  Otherwise a lane stores its own row, 32 bytes at a time.
+template <int BN, class T, bool STAGED>
 struct Wide {
     // warps that take the accumulators out: f32 outputs need room for a piece beside the sum
     static constexpr int kOut = sizeof(T) == 4 ? 16 : 8;
@@ -324,7 +343,8 @@ struct Wide {
     static constexpr int kThreads = 32 * (kOut + 3);
     static constexpr int kHalf = BN / 2;                       // weight rows per CTA
     static constexpr int kStageBytes = 128 * kTileK + kHalf * kTileK;
-    static constexpr int kStages = BN == 256 ? 6 : 8;
+    static constexpr int kStages = (BN == 256 ? 6 : 8) - (STAGED ? (BN == 128 && sizeof(T) == 4 ? 2 : 1) : 0);
+    static constexpr int kOutBytes = STAGED ? kOut * 32 * 17 * 4 : 0;      // 64 bytes of 32 rows per warp, 4 apart
     static constexpr int kSfBytes = 512 + 512 * (BN / 128);
     static constexpr int kSfCols = 4 + 4 * (BN / 128);
     static constexpr int kAcc = BN == 256 ? 1 : 2;             // accumulators in tensor memory
@@ -332,20 +352,16 @@ struct Wide {
     static constexpr int kBars = 2 * kStages + 2 * 2 + 2 * kAcc + 1;
     static constexpr int kCols = 512;
     static constexpr int kSmem = 227 * 1024;                   // all of an SM's, as all of its tensor memory
-    static_assert(1024 + kStages * kStageBytes + kSlots * kSfBytes + kRawA + kRawB + 8 * kBars + 16 <= kSmem, "shared memory");
+    static_assert(1024 + kStages * kStageBytes + kSlots * kSfBytes + kRawA + kRawB + kOutBytes + 8 * kBars + 16 <= kSmem, "shared memory");
     static_assert(kAcc * BN + kSlots * kSfCols <= kCols, "tensor memory");
 };
 
-// 32 bytes to one row of the output: the values of columns n.. (T of 2 or 4 bytes)
+// 32 bytes to a 32-byte-aligned place of one row of the output, `left` columns before its end
 template <class T>
 __device__ __forceinline__ void store_run(T* out, const uint32_t (&w)[8], int64_t left) {
     constexpr int kPer = 32 / sizeof(T);
-    const uintptr_t a = reinterpret_cast<uintptr_t>(out);
-    if (left >= kPer && (a & 31) == 0) {
+    if (left >= kPer) {
         stg256(out, w);
-    } else if (left >= kPer && (a & 15) == 0) {
-        stg128(out, make_uint4(w[0], w[1], w[2], w[3]));
-        stg128(reinterpret_cast<uint8_t*>(out) + 16, make_uint4(w[4], w[5], w[6], w[7]));
     } else {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
@@ -374,15 +390,15 @@ __device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int&
     tm = band * kBand + in - tn * tall;
 }
 
-template <int BN, class T>
-__global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
+template <int BN, class T, bool STAGED>
+__global__ void __launch_bounds__(Wide<BN, T, STAGED>::kThreads, 1)
     gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
                    const int tiles_m, const int tiles_n, const bool use_raw) {
-    using C = Wide<BN, T>;
+    using C = Wide<BN, T, STAGED>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
     const uint32_t sf = base + C::kStages * C::kStageBytes, raw_a = sf + C::kSlots * C::kSfBytes, raw_b = raw_a + kRawA;
-    const uint32_t bars = raw_b + kRawB, slot = bars + 8 * C::kBars;
+    const uint32_t out_stage = raw_b + kRawB, bars = out_stage + C::kOutBytes, slot = bars + 8 * C::kBars;
     const auto full = [&](int s) { return bars + 8 * s; };
     const auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
     const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
@@ -520,15 +536,61 @@ __global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
             }
             __syncwarp();
         };
+        const auto direct = [&](int64_t m0, int64_t nb0, int g0, uint32_t (&x)[kBatch][4], uint32_t (&w)[kBatch][kB]) {
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                const int kb = 4 * (g0 + u);
+                if (g0 + u >= groups) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int64_t m = m0 + 32 * j + lane;
+                    x[u][j] = m < p.m ? scale_word(p.a_scales + m * p.ld_a_scales, kb, blocks) : 0x7F7F7F7Fu;
+                }
+#pragma unroll
+                for (int j = 0; j < kB; ++j)
+                    w[u][j] = nb0 + j < nbs ? scale_word(p.b_scales + (nb0 + j) * p.ld_b_scales, kb, blocks) : 0x7F7F7F7Fu;
+            }
+        };
+        const auto stage = [&](int g0, const uint32_t (&x)[kBatch][4], const uint32_t (&w)[kBatch][kB]) {
+            if (bi > 1 && !(ok = tc::wait(sf_empty(bi & 1), ((bi >> 1) - 1) & 1))) return;
+#pragma unroll
+            for (int u = 0; u < kBatch; ++u) {
+                if (g0 + u >= groups) continue;
+                const uint32_t to = sf + ((bi & 1) * kBatch + u) * C::kSfBytes + 16 * lane;
+                sts(to, make_uint4(x[u][0], x[u][1], x[u][2], x[u][3]));
+#pragma unroll
+                for (int j = 0; j < kB; ++j) sts(to + 512 + 512 * j, make_uint4(w[u][j], w[u][j], w[u][j], w[u][j]));
+            }
+            tc::fence_async_shared();
+            __syncwarp();
+            if (lane == 0) tc::arrive_remote(tc::map_shared(sf_full(bi & 1), 0));
+            ++bi;
+        };
+        uint32_t x[kBatch][4], w[kBatch][kB];
+        if (groups <= kBatch) {
+            // short sums: one batch per tile, the next tile's on its way in registers
+            int tm, tn;
+            if (pair < tiles) {
+                tile_place(pair, tiles_m, tiles_n, tm, tn);
+                direct(static_cast<int64_t>(tm) * 256 + 128 * rank, static_cast<int64_t>(tn) * kB, 0, x, w);
+            }
+            for (int t = pair; t < tiles && ok; t += pairs) {
+                stage(0, x, w);
+                if (t + pairs < tiles) {
+                    tile_place(t + pairs, tiles_m, tiles_n, tm, tn);
+                    direct(static_cast<int64_t>(tm) * 256 + 128 * rank, static_cast<int64_t>(tn) * kB, 0, x, w);
+                }
+            }
+        }
         // the very first batch is read as it lies in global memory, ahead of the first tile loads
         if (use_raw && pair < tiles && groups > kBatch) request(pair);
-        for (int t = pair; t < tiles && ok; t += pairs) {
+        for (int t = pair; groups > kBatch && t < tiles && ok; t += pairs) {
             int tm, tn;
             tile_place(t, tiles_m, tiles_n, tm, tn);
             const int64_t m0 = static_cast<int64_t>(tm) * 256 + 128 * rank, nb0 = static_cast<int64_t>(tn) * kB;
             uint32_t from_a[4] = {0, 0, 0, 0}, from_b[kB] = {};
             bool raw = false;
-            for (int g0 = 0; g0 < groups; g0 += kBatch, ++bi) {
+            for (int g0 = 0; g0 < groups; g0 += kBatch) {
                 if (use_raw && !raw && bi > 0) {
                     if (!(ok = tc::wait(raw_full, read & 1))) break;
                     ++read;
@@ -541,23 +603,18 @@ __global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
 #pragma unroll
                     for (int j = 0; j < kB; ++j) from_b[j] = raw_b + rb.skew + static_cast<uint32_t>(j * p.ld_b_scales);
                 }
-                uint32_t x[kBatch][4], w[kBatch][kB];
+                if (raw) {
 #pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    const int kb = 4 * (g0 + u);
-                    if (g0 + u >= groups) continue;
+                    for (int u = 0; u < kBatch; ++u) {
+                        if (g0 + u >= groups) continue;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const int64_t m = m0 + 32 * j + lane;
-                        x[u][j] = m >= p.m ? 0x7F7F7F7Fu
-                                  : raw    ? raw_word(from_a[j] + kb, words)
-                                           : scale_word(p.a_scales + m * p.ld_a_scales, kb, blocks);
+                        for (int j = 0; j < 4; ++j)
+                            x[u][j] = m0 + 32 * j + lane < p.m ? raw_word(from_a[j] + 4 * (g0 + u), words) : 0x7F7F7F7Fu;
+#pragma unroll
+                        for (int j = 0; j < kB; ++j) w[u][j] = nb0 + j < nbs ? raw_word(from_b[j] + 4 * (g0 + u), words) : 0x7F7F7F7Fu;
                     }
-#pragma unroll
-                    for (int j = 0; j < kB; ++j)
-                        w[u][j] = nb0 + j >= nbs ? 0x7F7F7F7Fu
-                                  : raw          ? raw_word(from_b[j] + kb, words)
-                                                 : scale_word(p.b_scales + (nb0 + j) * p.ld_b_scales, kb, blocks);
+                } else {
+                    direct(m0, nb0, g0, x, w);
                 }
                 // this tile's are read: the next one's may overwrite them
                 if (use_raw && g0 + kBatch >= groups && t + pairs < tiles) {
@@ -565,18 +622,8 @@ __global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
                     __syncwarp();
                     request(t + pairs);
                 }
-                if (bi > 1 && !(ok = tc::wait(sf_empty(bi & 1), ((bi >> 1) - 1) & 1))) break;
-#pragma unroll
-                for (int u = 0; u < kBatch; ++u) {
-                    if (g0 + u >= groups) continue;
-                    const uint32_t to = sf + ((bi & 1) * kBatch + u) * C::kSfBytes + 16 * lane;
-                    sts(to, make_uint4(x[u][0], x[u][1], x[u][2], x[u][3]));
-#pragma unroll
-                    for (int j = 0; j < kB; ++j) sts(to + 512 + 512 * j, make_uint4(w[u][j], w[u][j], w[u][j], w[u][j]));
-                }
-                tc::fence_async_shared();
-                __syncwarp();
-                if (lane == 0) tc::arrive_remote(tc::map_shared(sf_full(bi & 1), 0));
+                stage(g0, x, w);
+                if (!ok) break;
             }
         }
         // a request that nothing waited for, after a wait that gave up
@@ -614,7 +661,7 @@ __global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
                 // the accumulators are free for the next piece once they are in registers
                 tc::fence_before();
                 __syncwarp();
-                if (lane == 0) tc::arrive_remote(tc::map_shared(acc_empty(b), 0));
+                if (lane == 0) tc::arrive_remote_relaxed(tc::map_shared(acc_empty(b), 0));
             }
             if (!ok) break;
             if (p.bias != nullptr) {
@@ -622,9 +669,37 @@ __global__ void __launch_bounds__(Wide<BN, T>::kThreads, 1)
                 for (int i = 0; i < kPart; ++i)
                     if (n0 + i < p.n) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), __ldg(p.bias + n0 + i)));
             }
-            if (m < p.m) {
+            constexpr int kPer = 32 / sizeof(T);
+            if constexpr (STAGED) {
+                // 64 bytes of each of the warp's rows at a time, two rows to a store
+                const uint32_t stage = out_stage + warp * (32 * 17 * 4);
+                const int64_t top = m - lane;
+#pragma unroll
+                for (int c = 0; c < kPart; c += 2 * kPer) {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        if constexpr (sizeof(T) == 4) sts(stage + 4 * (17 * lane + i), v[c + i]);
+                        else sts(stage + 4 * (17 * lane + i), pack2<T>(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1])));
+                    }
+                    __syncwarp();
+                    const int word = lane & 15;
+                    const int64_t col = n0 + c + word * static_cast<int>(4 / sizeof(T));
+                    T* out = reinterpret_cast<T*>(p.out) + (top + (lane >> 4)) * p.ld_out + col;
+#pragma unroll 4
+                    for (int r = lane >> 4; r < 32; r += 2, out += 2 * p.ld_out) {
+                        const uint32_t x = lds_u32(stage + 4 * (17 * r + word));
+                        if (top + r >= p.m || col >= p.n) continue;
+                        if (sizeof(T) == 4 || (col + 1 < p.n && (reinterpret_cast<uintptr_t>(out) & 3) == 0)) {
+                            st_global(reinterpret_cast<uint32_t*>(out), x);
+                        } else {
+                            st_global(reinterpret_cast<uint16_t*>(out), static_cast<uint16_t>(x));
+                            if (col + 1 < p.n) st_global(reinterpret_cast<uint16_t*>(out) + 1, static_cast<uint16_t>(x >> 16));
+                        }
+                    }
+                    __syncwarp();
+                }
+            } else if (m < p.m) {
                 T* const out = reinterpret_cast<T*>(p.out) + m * p.ld_out + n0;
-                constexpr int kPer = 32 / sizeof(T);
 #pragma unroll
                 for (int c = 0; c < kPart; c += kPer) {
                     uint32_t run[8];
@@ -689,10 +764,10 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
                         map_a, p, split);
 }
 
-template <int BN, class T>
+template <int BN, class T, bool STAGED>
 int launch_wide(const GqMatmul& p, cudaStream_t s) {
-    using C = Wide<BN, T>;
-    auto kern = gq_matmul_wide<BN, T>;
+    using C = Wide<BN, T, STAGED>;
+    auto kern = gq_matmul_wide<BN, T, STAGED>;
     CUtensorMap map_b, map_a;
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
         return static_cast<int>(cudaErrorInvalidValue);
@@ -711,7 +786,8 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
 
 // Which kernel and tile: the least estimated time (us).  A narrow tile costs what its operands
 // take through an SM's read path (133 KB a us), the busiest SM counts, and no less than reading
-// the operands from HBM (6.3 MB a us); set-up and the sums' way out grow with the tile.  A wide
+// the operands from HBM (6.3 MB a us); set-up and the sums' way out grow with the tile and come
+// again with every round of CTAs.  A wide
 // one costs its matrix instructions (0.287 us per 256 x 256 x 128 on a pair, 0.19 per 256 x 128 x
 // 128, where shared memory bounds it) and a drain, in rounds over the pairs.  Measured against
 // it (us, k = 4096 unless said; the best and the runner-up): 64 x 28672 narrow 64 23.1, narrow 128
@@ -735,7 +811,8 @@ int choose(const GqMatmul& p, bool f32) {
         if (f32 && bn == 128 && p.kb > 3 * kPiece / 2 * split) continue;      // a sum in one piece (see kPiece)
         const int64_t ctas = (p.m + bn - 1) / bn * ((p.n + 127) / 128) * split;
         const double bytes = static_cast<double>((ctas + sms - 1) / sms) * static_cast<double>((p.kb + split - 1) / split) * (128 + bn) * 128;
-        take(bn, 3.0 + 0.032 * bn + (split > 1 ? 1.0 : 0.0) + std::max(bytes / 133e3, hbm));
+        const double rounds = static_cast<double>((ctas + 2 * sms - 1) / (2 * sms));      // two CTAs on an SM
+        take(bn, rounds * (3.0 + 0.032 * bn) + (split > 1 ? 1.0 : 0.0) + std::max(bytes / 133e3, hbm));
     }
     for (int bn : {128, 256}) {
         const int64_t tiles = (p.m + 255) / 256 * ((p.n + bn - 1) / bn), pairs = sms / 2;
@@ -762,13 +839,14 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
         return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
+    const bool staged = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.m > 1 ? p.ld_out * sizeof(T) : 0)) % 32 != 0;
     switch (choose(p, sizeof(T) == 4)) {
         case 16: return launch_narrow<16, T>(p, s);
         case 32: return launch_narrow<32, T>(p, s);
         case 64: return launch_narrow<64, T>(p, s);
         case 128: return launch_narrow<128, T>(p, s);
-        case 2 * 128: return launch_wide<128, T>(p, s);
-        default: return launch_wide<256, T>(p, s);
+        case 2 * 128: return staged ? launch_wide<128, T, true>(p, s) : launch_wide<128, T, false>(p, s);
+        default: return staged ? launch_wide<256, T, true>(p, s) : launch_wide<256, T, false>(p, s);
     }
 }
 

@@ -112,6 +112,17 @@ __device__ __forceinline__ float4 load_cluster(uint32_t addr) {
 __device__ __forceinline__ void arrive_remote(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
+// The same without ordering the thread's memory accesses (a release waits for its stores to
+// global memory): for what tcgen05.fence orders
+__device__ __forceinline__ void arrive_remote_relaxed(uint32_t bar) {
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+
+__device__ __forceinline__ float load_cluster1(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
 
 // ---- a pair of CTAs working on one instruction (cta_group::2) --------------------------------
 

@@ -137,6 +137,7 @@ int float_bytes(int dtype) {
     }
 }
 
+constexpr int64_t kMaxExtent = INT32_MAX - 512;    // tile coordinates are 32-bit, a tile past the end included
 constexpr int64_t kMaxStride = int64_t(1) << 38;   // the limit of a tensor map's byte strides is 2^40
 
 int rows_check(int64_t rows, int64_t cols) {
@@ -603,7 +604,7 @@ int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64
     const int es = float_bytes(dtype);
     if (es == 0) return GQ_ERR_TYPE;
     if (m < 0 || n < 0 || k < 0 || k % 32 != 0) return GQ_ERR_SIZE;
-    if (m > INT32_MAX || n > INT32_MAX || k > INT32_MAX) return GQ_ERR_SIZE;
+    if (m > kMaxExtent || n > kMaxExtent || k > kMaxExtent) return GQ_ERR_SIZE;
     const int64_t kb = (k + 127) / 128;
     if (ld_a < k || ld_b < k || ld_a_scales < kb || ld_b_scales < kb || ld_out < n) return GQ_ERR_SIZE;
     if (ld_a > kMaxStride || ld_b > kMaxStride || ld_a_scales > kMaxStride || ld_b_scales > kMaxStride || ld_out > kMaxStride)

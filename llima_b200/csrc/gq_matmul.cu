@@ -332,10 +332,12 @@ __device__ __forceinline__ uint32_t raw_word(uint32_t raw, int off, int whole, c
     return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
 }
 
-// STAGED: outputs whose rows do not start on 32 bytes go out through shared memory, a row's values
-// side by side from neighbouring lanes; a stage of the ring (two for f32 in narrow tiles) makes
-// room.  Otherwise a lane stores its own row, 32 bytes at a time.
-template <int BN, class T, bool STAGED>
+// Outputs go out through shared memory, a few KB per warp, in the place of a stage of the ring
+// (measured: the ring loses nothing by it): as boxes of a tensor map where the rows start on 16
+// bytes, or (PLAIN) by the warp's own stores, a row's values side by side from neighbouring
+// lanes.  A lane that stores its own row directly touches 32 lines at a time (8192 x 28672 x 4096
+// 689 against 649 us without stores; 440 us for 6482 x 12260 x 320, whose rows start off 16 bytes).
+template <int BN, class T, bool PLAIN>
 struct Wide {
     // warps that take the accumulators out: f32 outputs need room for a piece beside the sum
     static constexpr int kOut = sizeof(T) == 4 ? 16 : 8;
@@ -343,8 +345,9 @@ struct Wide {
     static constexpr int kThreads = 32 * (kOut + 3);
     static constexpr int kHalf = BN / 2;                       // weight rows per CTA
     static constexpr int kStageBytes = 128 * kTileK + kHalf * kTileK;
-    static constexpr int kStages = (BN == 256 ? 6 : 8) - (STAGED ? (BN == 128 && sizeof(T) == 4 ? 2 : 1) : 0);
-    static constexpr int kOutBytes = STAGED ? kOut * 32 * 17 * 4 : 0;      // 64 bytes of 32 rows per warp, 4 apart
+    static constexpr int kStages = BN == 256 ? 5 : PLAIN && sizeof(T) == 4 ? 6 : 7;
+    static constexpr int kBox = sizeof(T) == 4 ? 64 : 128;     // bytes of a row that a warp stages at a time
+    static constexpr int kOutBytes = PLAIN ? kOut * 32 * 17 * 4 : kOut * 32 * kBox;
     static constexpr int kSfBytes = 512 + 512 * (BN / 128);
     static constexpr int kSfCols = 4 + 4 * (BN / 128);
     static constexpr int kAcc = BN == 256 ? 1 : 2;             // accumulators in tensor memory
@@ -352,25 +355,9 @@ struct Wide {
     static constexpr int kBars = 2 * kStages + 2 * 2 + 2 * kAcc + 1;
     static constexpr int kCols = 512;
     static constexpr int kSmem = 227 * 1024;                   // all of an SM's, as all of its tensor memory
-    static_assert(1024 + kStages * kStageBytes + kSlots * kSfBytes + kRawA + kRawB + kOutBytes + 8 * kBars + 16 <= kSmem, "shared memory");
+    static_assert(1024 + kStages * kStageBytes + kSlots * kSfBytes + kRawA + kRawB + kOutBytes + 128 + 8 * kBars + 16 <= kSmem, "shared memory");
     static_assert(kAcc * BN + kSlots * kSfCols <= kCols, "tensor memory");
 };
-
-// 32 bytes to a 32-byte-aligned place of one row of the output, `left` columns before its end
-template <class T>
-__device__ __forceinline__ void store_run(T* out, const uint32_t (&w)[8], int64_t left) {
-    constexpr int kPer = 32 / sizeof(T);
-    if (left >= kPer) {
-        stg256(out, w);
-    } else {
-#pragma unroll
-        for (int i = 0; i < kPer; ++i)
-            if (i < left) {
-                if constexpr (sizeof(T) == 4) reinterpret_cast<uint32_t*>(out)[i] = w[i];
-                else reinterpret_cast<uint16_t*>(out)[i] = static_cast<uint16_t>(w[i / 2] >> (16 * (i & 1)));
-            }
-    }
-}
 
 template <class T>
 __device__ __forceinline__ uint32_t pack2(float x, float y) {
@@ -390,15 +377,15 @@ __device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int&
     tm = band * kBand + in - tn * tall;
 }
 
-template <int BN, class T, bool STAGED>
-__global__ void __launch_bounds__(Wide<BN, T, STAGED>::kThreads, 1)
-    gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b, const GqMatmul p,
-                   const int tiles_m, const int tiles_n, const bool use_raw) {
-    using C = Wide<BN, T, STAGED>;
+template <int BN, class T, bool PLAIN>
+__global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
+    gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const __grid_constant__ CUtensorMap map_out, const GqMatmul p, const int tiles_m, const int tiles_n, const bool use_raw) {
+    using C = Wide<BN, T, PLAIN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
-    const uint32_t sf = base + C::kStages * C::kStageBytes, raw_a = sf + C::kSlots * C::kSfBytes, raw_b = raw_a + kRawA;
-    const uint32_t out_stage = raw_b + kRawB, bars = out_stage + C::kOutBytes, slot = bars + 8 * C::kBars;
+    const uint32_t out_stage = base + C::kStages * C::kStageBytes, sf = out_stage + (C::kOutBytes + 127) / 128 * 128;
+    const uint32_t raw_a = sf + C::kSlots * C::kSfBytes, raw_b = raw_a + kRawA, bars = raw_b + kRawB, slot = bars + 8 * C::kBars;
     const auto full = [&](int s) { return bars + 8 * s; };
     const auto empty = [&](int s) { return bars + 8 * (C::kStages + s); };
     const auto sf_full = [&](int s) { return bars + 8 * (2 * C::kStages + s); };
@@ -669,13 +656,12 @@ __global__ void __launch_bounds__(Wide<BN, T, STAGED>::kThreads, 1)
                 for (int i = 0; i < kPart; ++i)
                     if (n0 + i < p.n) v[i] = __float_as_uint(__fadd_rn(__uint_as_float(v[i]), __ldg(p.bias + n0 + i)));
             }
-            constexpr int kPer = 32 / sizeof(T);
-            if constexpr (STAGED) {
+            if constexpr (PLAIN) {
                 // 64 bytes of each of the warp's rows at a time, two rows to a store
                 const uint32_t stage = out_stage + warp * (32 * 17 * 4);
                 const int64_t top = m - lane;
 #pragma unroll
-                for (int c = 0; c < kPart; c += 2 * kPer) {
+                for (int c = 0; c < kPart; c += 64 / static_cast<int>(sizeof(T))) {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
                         if constexpr (sizeof(T) == 4) sts(stage + 4 * (17 * lane + i), v[c + i]);
@@ -698,20 +684,36 @@ __global__ void __launch_bounds__(Wide<BN, T, STAGED>::kThreads, 1)
                     }
                     __syncwarp();
                 }
-            } else if (m < p.m) {
-                T* const out = reinterpret_cast<T*>(p.out) + m * p.ld_out + n0;
+            } else {
+                // boxes of 32 rows x kBox bytes in the swizzle of that width: 16-byte piece j of
+                // row r at j ^ (r % 8) (128 bytes) or j ^ (r / 2 % 4) (64)
+                constexpr int kCols = C::kBox / static_cast<int>(sizeof(T));
+                const uint32_t stage = out_stage + warp * (32 * C::kBox), row = stage + lane * C::kBox;
+                const int turn = C::kBox == 128 ? lane & 7 : (lane >> 1) & 3;
+                const int64_t top = m - lane;
 #pragma unroll
-                for (int c = 0; c < kPart; c += kPer) {
-                    uint32_t run[8];
+                for (int c = 0; c < kPart; c += kCols) {
+                    if (tc::elect()) tc::store_read();      // the box before this one
+                    __syncwarp();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if constexpr (sizeof(T) == 4) run[i] = v[c + i];
-                        else run[i] = pack2<T>(__uint_as_float(v[c + 2 * i]), __uint_as_float(v[c + 2 * i + 1]));
+                    for (int j = 0; j < C::kBox / 16; ++j) {
+                        uint32_t x[4];
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            if constexpr (sizeof(T) == 4) x[k] = v[c + 4 * j + k];
+                            else x[k] = pack2<T>(__uint_as_float(v[c + 8 * j + 2 * k]), __uint_as_float(v[c + 8 * j + 2 * k + 1]));
+                        }
+                        sts(row + 16 * (j ^ turn), make_uint4(x[0], x[1], x[2], x[3]));
                     }
-                    store_run<T>(out + c, run, p.n - n0 - c);
+                    tc::fence_async_shared();
+                    __syncwarp();
+                    if (top < p.m && n0 + c < p.n && tc::elect())
+                        tc::store_tile(&map_out, static_cast<int>(n0 + c), static_cast<int>(top), stage);
                 }
             }
         }
+        if (!PLAIN && tc::elect()) tc::store_done();
+        __syncwarp();
     }
     if (!ok) atomicOr(&gq_matmul_errors, kErrWaitTimeout);
     __syncwarp();
@@ -764,13 +766,23 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
                         map_a, p, split);
 }
 
-template <int BN, class T, bool STAGED>
+template <int BN, class T, bool PLAIN>
 int launch_wide(const GqMatmul& p, cudaStream_t s) {
-    using C = Wide<BN, T, STAGED>;
-    auto kern = gq_matmul_wide<BN, T, STAGED>;
-    CUtensorMap map_b, map_a;
+    using C = Wide<BN, T, PLAIN>;
+    auto kern = gq_matmul_wide<BN, T, PLAIN>;
+    CUtensorMap map_b, map_a, map_out{};
     if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
         return static_cast<int>(cudaErrorInvalidValue);
+    if (!PLAIN) {
+        const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.n), static_cast<cuuint64_t>(p.m)};
+        const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ld_out) * sizeof(T)};
+        const cuuint32_t box[2] = {C::kBox / sizeof(T), 32}, step[2] = {1, 1};
+        if (encode_tiled()(&map_out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims,
+                           strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           C::kBox == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+            return static_cast<int>(cudaErrorInvalidValue);
+    }
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -780,7 +792,7 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
                          128 * p.ld_a_scales <= kRawA && BN / 128 * p.ld_b_scales + 32 <= kRawB;
     const int64_t pairs = sm_count() / 2;
     const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
-    return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, p, static_cast<int>(tiles_m),
+    return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, map_out, p, static_cast<int>(tiles_m),
                         static_cast<int>(tiles_n), use_raw);
 }
 
@@ -839,14 +851,14 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
         return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
-    const bool staged = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.m > 1 ? p.ld_out * sizeof(T) : 0)) % 32 != 0;
+    const bool plain = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T))) % 16 != 0;
     switch (choose(p, sizeof(T) == 4)) {
         case 16: return launch_narrow<16, T>(p, s);
         case 32: return launch_narrow<32, T>(p, s);
         case 64: return launch_narrow<64, T>(p, s);
         case 128: return launch_narrow<128, T>(p, s);
-        case 2 * 128: return staged ? launch_wide<128, T, true>(p, s) : launch_wide<128, T, false>(p, s);
-        default: return staged ? launch_wide<256, T, true>(p, s) : launch_wide<256, T, false>(p, s);
+        case 2 * 128: return plain ? launch_wide<128, T, true>(p, s) : launch_wide<128, T, false>(p, s);
+        default: return plain ? launch_wide<256, T, true>(p, s) : launch_wide<256, T, false>(p, s);
     }
 }
 

@@ -49,6 +49,17 @@ __device__ __forceinline__ void bulk(uint32_t dst, const void* src, int bytes, u
                  : "memory");
 }
 
+// A box in this CTA's shared memory to column x and row y of a 2-D tensor map; what lies outside
+// the tensor is left out.  store_read: until the thread's stores have read their boxes;
+// store_done: until they are complete.
+__device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(map),
+                 "r"(x), "r"(y), "r"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void store_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void store_done() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 __device__ __forceinline__ void arrive_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }

@@ -378,6 +378,43 @@ def test_product_strided_operands(m):
             assert bool((wide == 7.0).all())
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n", [2600, 2597, 2612])
+@pytest.mark.parametrize("k,layout", [(320, "plain"), (2080, "plain"), (2080, "offset"), (2080, "pitch"), (4128, "plain"), (17440, "plain")])
+def test_product_many_tiles(n, k, layout, dtype):
+    """More tiles than pairs of SMs, with sums of one and several batches of scales, rows of the
+    output on and off 16 bytes, and scales that lie side by side, off 16 bytes, or apart."""
+    m = 2500 if k < 10000 else 1900
+    a, w = operands(m, n, k, 31)
+    blocks = a.scales.shape[1]
+
+    def relay(t):
+        left, pitch = {"plain": (0, blocks), "offset": (3, blocks + 5), "pitch": (0, blocks + 7)}[layout]
+        wide = torch.full((t.shape[0] + 1, pitch), 0xFF, dtype=torch.uint8, device=DEV)
+        wide[:-1, left:left + blocks] = t.view(torch.uint8)
+        return wide[:-1, left:left + blocks].view(fp8.E8M0)
+
+    a, w = fp8.Fp8Rows(a.codes, relay(a.scales)), fp8.Fp8Weight(w.codes, relay(w.scales))
+    bias = torch.randn(n, device=DEV) if k == 2080 else None
+    check_product(fp8.matmul_fp8(a, w, bias=bias, dtype=dtype), a, w, bias)
+
+
+def test_scales_at_the_end_of_their_memory():
+    """Scales whose last byte is their allocation's last: nothing past them is read for a result."""
+    for m, n, k in ((2500, 2600, 2080), (2499, 2597, 4128), (130, 300, 1056)):
+        a, w = operands(m, n, k, 32)
+
+        def at_end(t):
+            room = -(-t.numel() // 512) * 512
+            buf = torch.full((room,), 0xFF, dtype=torch.uint8, device=DEV)
+            start = (room - t.numel()) // 16 * 16       # on 16 bytes, so that the bulk copies are taken
+            buf[start:start + t.numel()] = t.view(torch.uint8).reshape(-1)
+            return buf[start:start + t.numel()].view(t.shape).view(fp8.E8M0)
+
+        b, v = fp8.Fp8Rows(a.codes, at_end(a.scales)), fp8.Fp8Weight(w.codes, at_end(w.scales))
+        assert torch.equal(fp8.matmul_fp8(b, v, dtype=torch.float32), fp8.matmul_fp8(a, w, dtype=torch.float32))
+
+
 def test_product_nan_reaches_its_row_and_column_only():
     for m in (5, 300):
         a, w = operands(m, 200, 256, 4)
@@ -565,6 +602,47 @@ def test_captured_and_replayed(tmp_path, rows):
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+@pytest.mark.parametrize("m", [1, 40, 300, 1500])
+def test_back_to_back_on_the_same_buffers(m):
+    """Kernels of this module begin under the one before them: a chain that writes what the last
+    link still reads, over and over on the same buffers, gives what single calls give."""
+    w1, w2 = operands(1, 512, 1024, 40)[1], operands(1, 1024, 256, 41)[1]
+    norm = torch.randn(1024, device=DEV)
+    x0 = rows_of(m, 1024, torch.bfloat16, 42)
+
+    def links(x, out, wait):
+        q, h = fp8.rms_norm_fp8(x, norm, residual=x, **({} if out is None else {"out": out[0], "sum_out": out[1]}))
+        wait()
+        both = fp8.matmul_fp8(q, w1, out=None if out is None else out[2])
+        wait()
+        s = fp8.quantize_fp8(both[:, 256:], gate=both[:, :256], out=None if out is None else out[3])
+        wait()
+        fp8.matmul_fp8(s, w2, out=x)
+        wait()
+        return h
+
+    x = x0.clone()
+    want = []
+    for _ in range(6):
+        h = links(x, None, torch.cuda.synchronize)
+        want.append((x.clone(), h.clone()))
+    x = x0.clone()
+    q = fp8.Fp8Rows(torch.empty(m, 1024, dtype=fp8.E4M3, device=DEV), torch.empty(m, 8, dtype=fp8.E8M0, device=DEV))
+    s = fp8.Fp8Rows(torch.empty(m, 256, dtype=fp8.E4M3, device=DEV), torch.empty(m, 2, dtype=fp8.E8M0, device=DEV))
+    out = (q, torch.empty_like(x), torch.empty(m, 512, dtype=torch.bfloat16, device=DEV), s)
+    got = []
+    for _ in range(6):
+        h = links(x, out, lambda: None)
+        got.append((x.clone(), h.clone()))
+    for (xa, ha), (xb, hb) in zip(got, want):
+        assert torch.equal(xa, xb) and torch.equal(ha, hb)
+    # and with nothing but these kernels on the stream between the copies out
+    x.copy_(x0)
+    for _ in range(6):
+        links(x, out, lambda: None)
+    assert torch.equal(x, want[-1][0])
+
+
 @pytest.mark.parametrize("m", [1, 24, 600])
 def test_two_streams_at_once(m):
     """Products on two streams share nothing: each gives what it gives alone."""
@@ -581,6 +659,21 @@ def test_two_streams_at_once(m):
     for i in (0, 1):
         for g in got[i]:
             assert torch.equal(g, want[i])
+
+
+def test_a_wait_of_the_product_that_nothing_ends_gives_up(tmp_path):
+    import shutil
+    import subprocess
+    from pathlib import Path
+    from llima_b200.build import ARCH, CSRC
+    root = Path(__file__).resolve().parents[1]
+    so = tmp_path / "libwait.so"
+    subprocess.run([shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc", *ARCH, "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+                    f"-I{CSRC}", f"-I{root / 'include'}", "-o", str(so), str(root / "tests" / "cuda" / "tensor_wait_timeout.cu")],
+                   check=True, capture_output=True)
+    status, waited = ctypes.c_int(-1), ctypes.c_ulonglong(0)
+    assert ctypes.CDLL(str(so)).run_wait_never(ctypes.byref(status), ctypes.byref(waited)) == 0
+    assert status.value == 0 and 0.9e9 <= waited.value <= 5e9
 
 
 def test_no_kernel_reported_an_error():

@@ -127,7 +127,7 @@ __device__ __forceinline__ void encode32(const __half2* q, const float* A, const
                 x = make_float2(nan_unless_finite(x.x), nan_unless_finite(x.y));
                 y = make_float2(nan_unless_finite(y.x), nan_unless_finite(y.y));
             }
-            c[j] = e4m3x2(x.x, x.y) | (e4m3x2(y.x, y.y) << 16);
+            c[j] = e4m3x4(x.x, x.y, y.x, y.y);
         }
     }
 }
@@ -341,14 +341,15 @@ struct Elem<BF16> {
 
 // Eight values over the block scale to eight codes
 __device__ __forceinline__ uint2 encode8(const float (&x)[8], float inv) {
-    uint32_t c[4];
+    uint32_t c[2];
     const float2 s = make_float2(inv, inv);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 y = __fmul2_rn(make_float2(nan_unless_finite(x[2 * i]), nan_unless_finite(x[2 * i + 1])), s);
-        c[i] = e4m3x2(y.x, y.y);
+    for (int i = 0; i < 2; ++i) {
+        const float2 y = __fmul2_rn(make_float2(nan_unless_finite(x[4 * i]), nan_unless_finite(x[4 * i + 1])), s);
+        const float2 z = __fmul2_rn(make_float2(nan_unless_finite(x[4 * i + 2]), nan_unless_finite(x[4 * i + 3])), s);
+        c[i] = e4m3x4(y.x, y.y, z.x, z.y);
     }
-    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
+    return make_uint2(c[0], c[1]);
 }
 __device__ __forceinline__ uint32_t amax8(const float (&x)[8]) {
     uint32_t m = 0;
@@ -527,7 +528,7 @@ __device__ __forceinline__ uint4 quantize_block(float2 (&y)[8], uint32_t& byte) 
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 u = __fmul2_rn(y[2 * i], s), v = __fmul2_rn(y[2 * i + 1], s);
-        c[i] = e4m3x2(u.x, u.y) | (e4m3x2(v.x, v.y) << 16);
+        c[i] = e4m3x4(u.x, u.y, v.x, v.y);
     }
     return make_uint4(c[0], c[1], c[2], c[3]);
 }

@@ -38,15 +38,18 @@ __device__ __forceinline__ uint32_t scale_byte(uint32_t amax_bits) {
 // 2^-e of a scale byte (0..247), a normal number
 __device__ __forceinline__ float inverse_scale(uint32_t byte) { return __uint_as_float((254u - byte) << 23); }
 
-// Two values already divided by the scale to two codes (x in the low byte), round to nearest
-// even.  The conversion saturates, which no finite value here needs (|x| <= 448).
-__device__ __forceinline__ uint32_t e4m3x2(float x, float y) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(r) : "f"(x), "f"(y));
+// Values already divided by the scale to codes, round to nearest even.  The conversion
+// saturates, which no finite value here needs (|x| <= 448).
+// Four values to a word of four codes, the first in the low byte
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint32_t r;
+    asm("{ .reg .b16 lo, hi; cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1; cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3; mov.b32 %0, {lo, hi}; }"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
     return r;
 }
 
-// The same for any value: one that is not finite becomes the NaN code
+// What becomes the NaN code where a value is not finite (an infinity would saturate)
 __device__ __forceinline__ float nan_unless_finite(float x) {
     return (__float_as_uint(x) & 0x7FFFFFFFu) < kInfBits ? x : __uint_as_float(0x7FFFFFFFu);
 }

@@ -249,24 +249,38 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
                 const int n = (u & 31) + 32 * i;
                 if (n0 + n >= p.n) continue;
                 const uint32_t at = base + (r * 128 + n) * 4;
-                float v = 0.0f;
-                for (int s = 0; s < split; ++s)
-                    v = __fadd_rn(v, split > 1 ? tc::load_cluster1(tc::map_shared(at, s)) : *reinterpret_cast<const float*>(smem + (r * 128 + n) * 4));
+                float x[8] = {*reinterpret_cast<const float*>(smem + (r * 128 + n) * 4), 0, 0, 0, 0, 0, 0, 0};
+                if (split > 1)
+#pragma unroll
+                    for (int s = 0; s < 8; ++s)
+                        if (s < split) x[s] = tc::load_cluster1(tc::map_shared(at, s));
+                float v = x[0];
+#pragma unroll
+                for (int s = 1; s < 8; ++s)
+                    if (s < split) v = __fadd_rn(v, x[s]);
                 if (p.bias != nullptr) v = __fadd_rn(v, p.bias[n0 + n]);
                 out[(m0 + r) * p.ld_out + n0 + n] = out_cast<T>(v);
             }
             continue;
         }
         if (n0 + c >= p.n) continue;
-        float v[4] = {0, 0, 0, 0};
         const uint32_t at = base + (r * 128 + c) * 4;
-        for (int s = 0; s < split; ++s) {
-            const float4 x = split > 1 ? tc::load_cluster(tc::map_shared(at, s)) : *reinterpret_cast<const float4*>(smem + (r * 128 + c) * 4);
-            v[0] = __fadd_rn(v[0], x.x);
-            v[1] = __fadd_rn(v[1], x.y);
-            v[2] = __fadd_rn(v[2], x.z);
-            v[3] = __fadd_rn(v[3], x.w);
-        }
+        float4 x[8];
+        x[0] = *reinterpret_cast<const float4*>(smem + (r * 128 + c) * 4);
+        // all CTAs' parts on their way before the first addition
+        if (split > 1)
+#pragma unroll
+            for (int s = 0; s < 8; ++s)
+                if (s < split) x[s] = tc::load_cluster(tc::map_shared(at, s));
+        float v[4] = {x[0].x, x[0].y, x[0].z, x[0].w};
+#pragma unroll
+        for (int s = 1; s < 8; ++s)
+            if (s < split) {
+                v[0] = __fadd_rn(v[0], x[s].x);
+                v[1] = __fadd_rn(v[1], x[s].y);
+                v[2] = __fadd_rn(v[2], x[s].z);
+                v[3] = __fadd_rn(v[3], x[s].w);
+            }
         if (p.bias != nullptr)
 #pragma unroll
             for (int i = 0; i < 4; ++i)

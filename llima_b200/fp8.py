@@ -93,6 +93,11 @@ def _matrix(t: torch.Tensor, name: str, dtype, device: int, rows: int | None = N
     return s0
 
 
+def _new(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """An uninitialized row-major tensor (empty_strided: the cheapest of torch's ways)."""
+    return torch.empty_strided((rows, cols), (cols, 1), dtype=dtype, device=device)
+
+
 def _device_of(t: torch.Tensor, name: str) -> int:
     if not t.is_cuda:
         raise TypeError(f"{name} must be a CUDA tensor")
@@ -121,7 +126,7 @@ def _rows_out(x: torch.Tensor, device: int, out: Fp8Rows | None):
     blocks = (cols + 127) >> 7
     if out is None:
         return (torch.empty_like(x, dtype=E4M3, memory_format=torch.contiguous_format), cols,
-                x.new_empty((rows, blocks), dtype=E8M0), blocks)
+                _new(rows, blocks, E8M0, x.device), blocks)
     codes, scales = out
     return (codes, _matrix(codes, "out.codes", E4M3, device, rows, cols),
             scales, _matrix(scales, "out.scales", E8M0, device, rows, blocks))
@@ -140,7 +145,7 @@ def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads:
     if out is None:
         if rows < 0 or cols < 0:
             raise ValueError(f"negative shape ({rows}, {cols})")
-        out = Fp8Weight(src.new_empty((rows, cols), dtype=E4M3), src.new_empty(shape, dtype=E8M0))
+        out = Fp8Weight(_new(rows, cols, E4M3, src.device), _new(*shape, E8M0, src.device))
     else:
         _matrix(out.codes, "out.codes", E4M3, dev, rows, cols)
         _matrix(out.scales, "out.scales", E8M0, dev, *shape)
@@ -231,7 +236,7 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     if out is None:
         if dtype not in _TYPE_IDS:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
-        out, ld_o = codes.new_empty((m, n), dtype=dtype), n
+        out, ld_o = _new(m, n, dtype, codes.device), n
     else:
         dtype = out.dtype
         if dtype not in _TYPE_IDS:

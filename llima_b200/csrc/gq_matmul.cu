@@ -8,7 +8,9 @@
 // that a few tokens cost a narrow instruction and not a padded one.  What bounds it is the
 // weights' traffic: a CTA streams its 128 rows through a ring of 128-column tiles.  Where
 // there are too few row tiles for the SMs, a cluster of 2 to 8 CTAs splits k and adds the
-// partial sums over distributed shared memory in a fixed order.
+// partial sums over distributed shared memory in a fixed order.  Measured: 1 x 28672 x 4096 in
+// 20.4 us (5.75 TB/s, 88% of the copy rate), 1 x 4096 x 4096 in 6.1 us, of which the weights'
+// bytes are 2.6 and the rest set-up, one round of loads and the join.
 #include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -303,7 +305,8 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
 // the weights' rows, so a pair reads as much from L2 as one CTA with a tile half as wide.
 // The first 8 warps (16 for f32 outputs) drain the accumulators into registers, release them and
 // then store; of the last three, one loads tiles, one (of the first CTA) issues the matrix
-// instructions and one stages the scales.
+// instructions and one stages the scales.  Measured: 8192 x 28672 x 4096 in 680 us (2.8 PFLOP/s)
+// in runs of a few ms; held for a second the board's 1000 W bring it to 780-880 us.
 
 // A tile's scales as they lie in memory: 128 rows of the tokens' and two of the weights', for all
 // of k.  They come by bulk copies, the next tile's as soon as this one's are read: the tile loads
@@ -338,13 +341,6 @@ __device__ __forceinline__ uint32_t raw_word(uint32_t a, bool words) {
 // columns), two batches in turn: the fence and the remote arrival that a batch ends with take
 // longer than the instructions of one group of a narrow tile.
 constexpr int kBatch = 4;
-
-// Four scale bytes at `off` of a region whose first `whole` bytes are in shared memory at `raw`
-__device__ __forceinline__ uint32_t raw_word(uint32_t raw, int off, int whole, const uint8_t* row, int64_t kb, int64_t blocks) {
-    if (off + 4 > whole) return scale_word(row, kb, blocks);
-    const uint32_t a = raw + off;
-    return __funnelshift_r(lds_u32(a & ~3u), lds_u32((a & ~3u) + 4), 8 * (a & 3u));
-}
 
 // Outputs go out through shared memory, a few KB per warp, in the place of a stage of the ring
 // (measured: the ring loses nothing by it): as boxes of a tensor map where the rows start on 16
@@ -381,20 +377,23 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
     return w;
 }
 
-// Tile t of the order in which pairs take them: bands of 8 row tiles, within a band column by
-// column, so that the tiles in flight share rows of both operands in L2.
-__device__ __forceinline__ void tile_place(int t, int tiles_m, int tiles_n, int& tm, int& tn) {
-    constexpr int kBand = 8;
-    const int band = t / (kBand * tiles_n), in = t - band * (kBand * tiles_n);
-    const int tall = min(kBand, tiles_m - band * kBand);
+// Tile t of the order in which pairs take them: bands of `tall` row tiles, within a band column by
+// column, so that the tiles in flight share rows of both operands in L2 and the band's tokens
+// stay there while the weights pass.
+struct Order {
+    int tiles_m, tiles_n, tall;
+};
+__device__ __forceinline__ void tile_place(int t, const Order& o, int& tm, int& tn) {
+    const int band = t / (o.tall * o.tiles_n), in = t - band * (o.tall * o.tiles_n);
+    const int tall = min(o.tall, o.tiles_m - band * o.tall);
     tn = in / tall;
-    tm = band * kBand + in - tn * tall;
+    tm = band * o.tall + in - tn * tall;
 }
 
 template <int BN, class T, bool PLAIN>
 __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
     gq_matmul_wide(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
-                   const __grid_constant__ CUtensorMap map_out, const GqMatmul p, const int tiles_m, const int tiles_n, const bool use_raw) {
+                   const __grid_constant__ CUtensorMap map_out, const GqMatmul p, const Order order, const bool use_raw) {
     using C = Wide<BN, T, PLAIN>;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t base = (smem_u32addr(smem_raw) + 1023u) & ~1023u;
@@ -410,7 +409,7 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
     const int tid = threadIdx.x, lane = tid & 31;
     const int warp = __shfl_sync(0xffffffffu, tid >> 5, 0);   // uniform for the compiler
     const uint32_t rank = tc::cluster_rank();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = tiles_m * tiles_n;
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1, tiles = order.tiles_m * order.tiles_n;
     const int blocks = static_cast<int>(p.kb), groups = (blocks + 3) / 4;
     if (warp == C::kOut + 1) tc::tmem_alloc_pair<C::kCols>(slot);
     if (warp == C::kOut && tc::elect()) {
@@ -446,7 +445,7 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
         int it = 0;
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
-            tile_place(t, tiles_m, tiles_n, tm, tn);
+            tile_place(t, order, tm, tn);
             const int m0 = tm * 256 + 128 * static_cast<int>(rank), n0 = tn * BN + C::kHalf * static_cast<int>(rank);
             for (int i = 0; i < blocks; ++i, ++it) {
                 const int s = it % C::kStages, round = it / C::kStages;
@@ -527,7 +526,7 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
         const auto request = [&](int t) {
             ++asked;
             int tm, tn;
-            tile_place(t, tiles_m, tiles_n, tm, tn);
+            tile_place(t, order, tm, tn);
             ra = raw_region(static_cast<int64_t>(tm) * 256 + 128 * rank, 128, p.m, p.ld_a_scales, p.kb);
             rb = raw_region(static_cast<int64_t>(tn) * kB, kB, nbs, p.ld_b_scales, p.kb);
             if (tc::elect()) {
@@ -572,13 +571,13 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
             // short sums: one batch per tile, the next tile's on its way in registers
             int tm, tn;
             if (pair < tiles) {
-                tile_place(pair, tiles_m, tiles_n, tm, tn);
+                tile_place(pair, order, tm, tn);
                 direct(static_cast<int64_t>(tm) * 256 + 128 * rank, static_cast<int64_t>(tn) * kB, 0, x, w);
             }
             for (int t = pair; t < tiles && ok; t += pairs) {
                 stage(0, x, w);
                 if (t + pairs < tiles) {
-                    tile_place(t + pairs, tiles_m, tiles_n, tm, tn);
+                    tile_place(t + pairs, order, tm, tn);
                     direct(static_cast<int64_t>(tm) * 256 + 128 * rank, static_cast<int64_t>(tn) * kB, 0, x, w);
                 }
             }
@@ -587,7 +586,7 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
         if (use_raw && pair < tiles && groups > kBatch) request(pair);
         for (int t = pair; groups > kBatch && t < tiles && ok; t += pairs) {
             int tm, tn;
-            tile_place(t, tiles_m, tiles_n, tm, tn);
+            tile_place(t, order, tm, tn);
             const int64_t m0 = static_cast<int64_t>(tm) * 256 + 128 * rank, nb0 = static_cast<int64_t>(tn) * kB;
             uint32_t from_a[4] = {0, 0, 0, 0}, from_b[kB] = {};
             bool raw = false;
@@ -635,7 +634,7 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
         int n = 0;
         for (int t = pair; t < tiles && ok; t += pairs) {
             int tm, tn;
-            tile_place(t, tiles_m, tiles_n, tm, tn);
+            tile_place(t, order, tm, tn);
             const int64_t m = static_cast<int64_t>(tm) * 256 + 128 * rank + 32 * (warp & 3) + lane;
             const int64_t n0 = static_cast<int64_t>(tn) * BN + kPart * (warp >> 2);
             uint32_t v[kPart];
@@ -806,8 +805,12 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
                          128 * p.ld_a_scales <= kRawA && BN / 128 * p.ld_b_scales + 32 <= kRawB;
     const int64_t pairs = sm_count() / 2;
     const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
-    return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, map_out, p, static_cast<int>(tiles_m),
-                        static_cast<int>(tiles_n), use_raw);
+    // a band's tokens take about 37 MB (measured, held for a second: 8192 x 28672 x 4096 819 / 783 /
+    // 756 / 756 us with bands of 4 / 8 / 16 / 32 tiles, 17 to 33 MB; 16384 x 8192 x 8192 857 / 852 / 866 /
+    // 949 with 12 / 16 / 20 / 32, the last 67 MB; 8192 x 4096 x 14336 395 / 404 / 430 with 12 / 16 / 32)
+    Order order{static_cast<int>(tiles_m), static_cast<int>(tiles_n), 0};
+    order.tall = static_cast<int>(std::min<int64_t>(std::max<int64_t>((int64_t(37) << 20) / (256 * p.k), 8), 32));
+    return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, map_out, p, order, use_raw);
 }
 
 // Which kernel and tile: the least estimated time (us).  A narrow tile costs what its operands

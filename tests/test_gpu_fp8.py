@@ -468,6 +468,49 @@ def test_product_repeats_bit_for_bit(m, n, k):
         assert torch.equal(fp8.matmul_fp8(a, w, dtype=torch.float32), first)
 
 
+# ---- past 32 bits ---------------------------------------------------------------------------
+
+
+def test_rows_past_32_bits():
+    """More than 2^31 values: the last rows come out as they do on their own."""
+    rows, cols = 527_000, 4096
+    x = torch.randn(1000, cols, device=DEV).bfloat16().repeat(rows // 1000, 1)
+    x[-5:] *= torch.arange(1, 6, device=DEV)[:, None].bfloat16()
+    w = torch.randn(cols, device=DEV)
+    for call in (fp8.quantize_fp8, lambda t: fp8.rms_norm_fp8(t, w)):
+        q, tail = call(x), call(x[-70:].clone())
+        assert torch.equal(q.codes[-70:].view(torch.uint8), tail.codes.view(torch.uint8))
+        assert torch.equal(q.scales[-70:].view(torch.uint8), tail.scales.view(torch.uint8))
+        del q
+    q, h = fp8.rms_norm_fp8(x, w, residual=x, sum_out=x)
+    del q
+    assert torch.equal(h[1000:1010], h[:10]) and torch.equal(h[-1005:-1000], h[-2005:-2000])
+
+
+def test_weight_past_32_bits():
+    rows, cols = 131_200, 16_416
+    size = cols // 32 * 18
+    raw = torch.randint(0, 256, (rows, size), dtype=torch.uint8, device=DEV)
+    raw.view(rows, -1, 18)[:, :, 0:2] = torch.tensor([0x66, 0x1C], dtype=torch.uint8, device=DEV)      # an ordinary f16
+    w = fp8.convert_fp8_device("Q4_0", raw.view(-1), rows, cols)
+    tail = fp8.convert_fp8_device("Q4_0", raw[-256:].reshape(-1).clone(), 256, cols)
+    assert torch.equal(w.codes[-256:].view(torch.uint8), tail.codes.view(torch.uint8))
+    assert torch.equal(w.scales[-2:].view(torch.uint8), tail.scales.view(torch.uint8))
+    # and as an operand
+    a = operands(3, 1, cols, 50)[0]
+    out = fp8.matmul_fp8(a, w, dtype=torch.float32)
+    check_product(out[:, -256:], a, tail)
+
+
+@pytest.mark.parametrize("n", [32_768, 32_765])
+def test_product_past_32_bits(n):
+    m, k = 66_000, 160
+    a, w = operands(m, n, k, 51)
+    out = fp8.matmul_fp8(a, w)
+    tail = fp8.Fp8Rows(a.codes[-300:], a.scales[-300:])
+    check_product(out[-300:], tail, w)
+
+
 # ---- refusals of the Python layer -----------------------------------------------------------
 
 
@@ -600,6 +643,45 @@ def test_captured_and_replayed(tmp_path, rows):
         got = y.clone(), h.clone()
         want = ffn(x, r)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+def test_captured_with_copies_and_a_fork():
+    """A graph in which these kernels follow a copy, a fill, each other on two streams, and the
+    join of both."""
+    a, w = operands(200, 512, 1024, 60)
+    _, v = operands(1, 1024, 512, 61)
+    host = torch.randn(200, 1024).bfloat16().pin_memory()
+    x = torch.empty(200, 1024, dtype=torch.bfloat16, device=DEV)
+    ones = torch.ones(1024, device=DEV)
+
+    def work(side):
+        main = torch.cuda.current_stream()
+        x.copy_(host, non_blocking=True)
+        q = fp8.rms_norm_fp8(x, ones)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            left = fp8.matmul_fp8(q, w)
+            left_q = fp8.quantize_fp8(left)
+        right = fp8.matmul_fp8(q, w, dtype=torch.float16)
+        right.zero_()
+        right_q = fp8.quantize_fp8(right)
+        main.wait_stream(side)
+        both = fp8.matmul_fp8(left_q, v, dtype=torch.float32)
+        return both, fp8.matmul_fp8(right_q, v), left
+
+    side = torch.cuda.Stream()
+    want = [t.clone() for t in work(side)]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = work(side)
+    for _ in range(3):
+        for t in got:
+            t.fill_(7)
+        graph.replay()
+        torch.cuda.synchronize()
+        for g, t in zip(got, want):
+            assert torch.equal(g, t)
 
 
 @pytest.mark.parametrize("m", [1, 40, 300, 1500])

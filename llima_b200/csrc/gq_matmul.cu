@@ -119,7 +119,9 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
     const int64_t m0 = tile % m_tiles * BN, n0 = tile / m_tiles * 128;
     const int kb0 = static_cast<int>(p.kb * rank / split), kb1 = static_cast<int>(p.kb * (rank + 1) / split);
     const int blocks = kb1 - kb0;
-    const int pieces = min(C::kPieces, (blocks + kPiece - 1) / kPiece), piece = (blocks + pieces - 1) / pieces;
+    // pieces of whole groups of four blocks
+    const int most = min(C::kPieces, (blocks + kPiece - 1) / kPiece), piece = ((blocks + most - 1) / most + 3) & ~3;
+    const int pieces = (blocks + piece - 1) / piece;
 
     if (warp == 5) tc::tmem_alloc<C::kCols>(slot);
     if (warp == 4 && tc::elect()) {
@@ -163,30 +165,45 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
         if (!ok)
             for (int i = max(0, issued - C::kStages); i < issued; ++i) tc::wait(full(i % C::kStages), (i / C::kStages) & 1);
     } else if (warp == 5) {
-        for (int i = 0; i < blocks; ++i) {
-            const int s = i % C::kStages, g = i / 4, q = g % kSfSlots;
-            const uint32_t ta = tmem + C::kPieces * BN + 8 * q, tb = ta + 4;
-            if (i % 4 == 0) {
-                if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
-                tc::fence_after();
-                if (tc::elect()) {
-                    tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
-                    tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
-                }
-                __syncwarp();
-            }
-            if (!(ok = tc::wait(full(s), (i / C::kStages) & 1))) break;
+        // what changes from block to block changes by additions: the loop's own instructions, not
+        // the matrix ones, set the pace of a narrow tile
+        const uint64_t da0 = tc::operand_desc(base), db0 = tc::operand_desc(base + 128 * kTileK);
+        uint64_t da = da0, db = db0;
+        uint32_t parity = 0;
+        int s = 0;
+        for (int g = 0; 4 * g < blocks && ok; ++g) {
+            const int q = g % kSfSlots;
+            const uint32_t d = tmem + BN * (4 * g / piece), ta = tmem + C::kPieces * BN + 8 * q, tb = ta + 4;
+            const bool first = 4 * g % piece == 0;
+            if (!(ok = tc::wait(sf_full(q), (g / kSfSlots) & 1))) break;
             tc::fence_after();
             if (tc::elect()) {
-                const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
-                const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
-                const uint32_t idesc = tc::instruction<128, BN>(i % 4);
-#pragma unroll
-                for (int k = 0; k < 4; ++k)
-                    tc::mma(tmem + BN * (i / piece), da + 2 * k, db + 2 * k, idesc, ta, tb, i % piece > 0 || k > 0);
-                tc::commit(empty(s));
-                if (i % 4 == 3 || i + 1 == blocks) tc::commit(sf_empty(q));
+                tc::copy_scales(ta, tc::scale_desc(sf + q * C::kSfBytes));
+                tc::copy_scales(tb, tc::scale_desc(sf + q * C::kSfBytes + 512));
             }
+            __syncwarp();
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (4 * g + u >= blocks || !ok) continue;
+                if (!(ok = tc::wait(full(s), parity))) continue;
+                tc::fence_after();
+                if (tc::elect()) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        tc::mma(d, da + 2 * k, db + 2 * k, tc::instruction<128, BN>(u), ta, tb, !first || u > 0 || k > 0);
+                    tc::commit(empty(s));
+                }
+                __syncwarp();
+                da += C::kStageBytes >> 4;
+                db += C::kStageBytes >> 4;
+                if (++s == C::kStages) {
+                    s = 0;
+                    parity ^= 1;
+                    da = da0;
+                    db = db0;
+                }
+            }
+            if (ok && tc::elect()) tc::commit(sf_empty(q));
             __syncwarp();
         }
         if (tc::elect()) tc::commit(done);
@@ -469,49 +486,65 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
             for (const uint64_t t0 = global_ns(); global_ns() - t0 < 10000000ull;) {
             }
     } else if (warp == C::kOut + 1) {
-        int it = 0, bi = 0, n = 0;     // blocks, batches and pieces so far
+        // what changes from block to block changes by additions: with divisions in it this loop
+        // took longer than a 256 x 128 tile's instructions (512 x 4096 x 14336 35 us)
+        constexpr int kPieceGroups = C::kPieceBlocks / 4;
+        const uint64_t da0 = tc::operand_desc(base), db0 = tc::operand_desc(base + 128 * kTileK);
+        uint64_t da = da0, db = db0;
+        uint32_t parity = 0;
+        int s = 0, bi = 0, n = 0;     // stage; batches and pieces so far
         for (int t = pair; rank == 0 && t < tiles && ok; t += pairs) {
-            for (int i = 0, j = 0; i < blocks; ++i, ++it) {      // j: the block's number in its piece
+            for (int g = 0; g < groups && ok; ++g) {
                 const int b = n % C::kAcc, use = n / C::kAcc;
-                if (j == 0) {
+                const bool first = g % kPieceGroups == 0;
+                if (first) {
                     if (use > 0 && !(ok = tc::wait(acc_empty(b), (use - 1) & 1))) break;
                     tc::fence_after();
                 }
-                const int s = it % C::kStages, q = (bi & 1) * kBatch + i / 4 % kBatch;
-                const uint32_t ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
-                if (i % (4 * kBatch) == 0) {
+                if (g % kBatch == 0) {
                     if (!(ok = tc::wait(sf_full(bi & 1), (bi >> 1) & 1))) break;
                     tc::fence_after();
                 }
-                if (i % 4 == 0) {
-                    if (tc::elect()) {
-                        const uint32_t from = sf + q * C::kSfBytes;
-                        tc::copy_scales_pair(ta, tc::scale_desc(from));
-#pragma unroll
-                        for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
-                    }
-                    __syncwarp();
-                }
-                if (!(ok = tc::wait(full(s), (it / C::kStages) & 1))) break;
-                tc::fence_after();
-                const bool last = i % (4 * kBatch) == 4 * kBatch - 1 || i + 1 == blocks;
+                const int q = (bi & 1) * kBatch + g % kBatch;
+                const uint32_t d = tmem + BN * b, ta = tmem + C::kAcc * BN + C::kSfCols * q, tb = ta + 4;
                 if (tc::elect()) {
-                    const uint64_t da = tc::operand_desc(base + s * C::kStageBytes);
-                    const uint64_t db = tc::operand_desc(base + s * C::kStageBytes + 128 * kTileK);
-                    const uint32_t idesc = tc::instruction<256, BN>(i % 4);
+                    const uint32_t from = sf + q * C::kSfBytes;
+                    tc::copy_scales_pair(ta, tc::scale_desc(from));
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) tc::mma_pair(tmem + BN * b, da + 2 * k, db + 2 * k, idesc, ta, tb, j > 0 || k > 0);
-                    tc::commit_pair(empty(s));
-                    if (last) tc::commit_pair(sf_empty(bi & 1));
+                    for (int j = 0; j < BN / 128; ++j) tc::copy_scales_pair(tb + 4 * j, tc::scale_desc(from + 512 + 512 * j));
                 }
                 __syncwarp();
-                if (last) ++bi;
-                if (++j == C::kPieceBlocks || i + 1 == blocks) {
-                    if (tc::elect()) tc::commit_pair(acc_full(b));
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    if (4 * g + u >= blocks || !ok) continue;
+                    if (!(ok = tc::wait(full(s), parity))) continue;
+                    tc::fence_after();
+                    if (tc::elect()) {
+#pragma unroll
+                        for (int k = 0; k < 4; ++k)
+                            tc::mma_pair(d, da + 2 * k, db + 2 * k, tc::instruction<256, BN>(u), ta, tb, !first || u > 0 || k > 0);
+                        tc::commit_pair(empty(s));
+                    }
                     __syncwarp();
-                    j = 0;
-                    ++n;
+                    da += C::kStageBytes >> 4;
+                    db += C::kStageBytes >> 4;
+                    if (++s == C::kStages) {
+                        s = 0;
+                        parity ^= 1;
+                        da = da0;
+                        db = db0;
+                    }
                 }
+                if (!ok) break;
+                const bool batch = g % kBatch == kBatch - 1 || g + 1 == groups;
+                const bool piece = g % kPieceGroups == kPieceGroups - 1 || g + 1 == groups;
+                if (tc::elect()) {
+                    if (batch) tc::commit_pair(sf_empty(bi & 1));
+                    if (piece) tc::commit_pair(acc_full(b));
+                }
+                __syncwarp();
+                bi += batch;
+                n += piece;
             }
             // after a wait that gave up: those who wait for this piece end sooner
             if (!ok && tc::elect()) tc::commit_pair(acc_full(n % C::kAcc));

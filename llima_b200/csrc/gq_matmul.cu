@@ -9,7 +9,7 @@
 // weights' traffic: a CTA streams its 128 rows through a ring of 128-column tiles.  Where
 // there are too few row tiles for the SMs, a cluster of 2 to 8 CTAs splits k and adds the
 // partial sums over distributed shared memory in a fixed order.  Measured: 1 x 28672 x 4096 in
-// 20.4 us (5.75 TB/s, 88% of the copy rate), 1 x 4096 x 4096 in 6.1 us, of which the weights'
+// 20.2 us (5.8 TB/s, 89% of the copy rate), 1 x 4096 x 4096 in 6.0 us, of which the weights'
 // bytes are 2.6 and the rest set-up, one round of loads and the join.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
 // the weights' rows, so a pair reads as much from L2 as one CTA with a tile half as wide.
 // The first 8 warps (16 for f32 outputs) drain the accumulators into registers, release them and
 // then store; of the last three, one loads tiles, one (of the first CTA) issues the matrix
-// instructions and one stages the scales.  Measured: 8192 x 28672 x 4096 in 680 us (2.8 PFLOP/s)
-// in runs of a few ms; held for a second the board's 1000 W bring it to 780-880 us.
+// instructions and one stages the scales.  Measured: 8192 x 28672 x 4096 in 656 us (2.9 PFLOP/s)
+// in runs of a few ms; held for a second the board's 1000 W bring it to 750-800 us.
 
 // A tile's scales as they lie in memory: 128 rows of the tokens' and two of the weights', for all
 // of k.  They come by bulk copies, the next tile's as soon as this one's are read: the tile loads
@@ -363,7 +363,7 @@ constexpr int kBatch = 4;
 // (measured: the ring loses nothing by it): as boxes of a tensor map where the rows start on 16
 // bytes, or (PLAIN) by the warp's own stores, a row's values side by side from neighbouring
 // lanes.  A lane that stores its own row directly touches 32 lines at a time (8192 x 28672 x 4096
-// 689 against 649 us without stores; 440 us for 6482 x 12260 x 320, whose rows start off 16 bytes).
+// 689 us against 649 without stores; 440 us for 6482 x 12260 x 320, whose rows start off 16 bytes).
 template <int BN, class T, bool PLAIN>
 struct Wide {
     // warps that take the accumulators out: f32 outputs need room for a piece beside the sum
@@ -857,12 +857,13 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
 // take through an SM's read path (133 KB a us), the busiest SM counts, and no less than reading
 // the operands from HBM (6.3 MB a us); set-up and the sums' way out grow with the tile and come
 // again with every round of CTAs.  A wide
-// one costs its matrix instructions (0.287 us per 256 x 256 x 128 on a pair, 0.19 per 256 x 128 x
-// 128, where shared memory bounds it) and a drain, in rounds over the pairs.  Measured against
-// it (us, k = 4096 unless said; the best and the runner-up): 64 x 28672 narrow 64 23.1, narrow 128
-// 24.1; 96 x 28672 narrow 128 25.4, wide 256 30.7; 160 x 28672 wide 256 31.9, wide 128 34.5; 128 x
-// 4096 narrow 64 9.0, narrow 128 11.6; 512 x 4096 wide 128 13.4, narrow 64 14.3; 768 x 4096 wide 256
-// 19.0, wide 128 19.9; 160 x 4096, k = 14336 narrow 128 19.9, narrow 64 23.6.
+// one costs its tiles (0.287 us per 256 x 256 x 128 on a pair, the matrix instructions' rate; 0.19 per
+// 256 x 128 x 128, where the way from the L2 bounds it: 24 KB per SM) and a drain, in rounds over
+// the pairs.  Measured against it (us, k = 4096 unless said; the best and the runner-up): 64 x 28672
+// narrow 64 23.2, narrow 128 24.7; 96 x 28672 narrow 128 26.1, wide 256 30.3; 160 x 28672 wide 256
+// 31.5, wide 128 33.8; 128 x 4096 narrow 64 9.0, wide 128 11.0; 512 x 4096 wide 128 12.0, narrow 64
+// 14.6; 768 x 4096 wide 256 16.8, wide 128 17.5; 160 x 4096, k = 14336 narrow 128 20.4, narrow 64
+// 24.0.  At most 1.11 times the best over 27 such shapes (512 x 4096, k = 512: 6.2 against 5.6).
 // Returns the narrow tile's tokens, or twice the wide tile's output channels.
 int choose(const GqMatmul& p, bool f32) {
     const int sms = sm_count();

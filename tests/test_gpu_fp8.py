@@ -353,6 +353,15 @@ def test_product_full_size(m, n, k):
     check_product(fp8.matmul_fp8(a, w, dtype=torch.float32), a, w)
 
 
+# more weight rows than one tile per SM holds, so that k is not split: sums of 34, 67 and 99 blocks
+# in two to four pieces, whose ends do not fall on a group of four
+@pytest.mark.parametrize("m,n,k", [(3, 19100, 4256), (20, 19100, 4256), (50, 19100, 4256), (3, 19100, 8480), (50, 19100, 8480),
+                                   (20, 19100, 12672), (600, 2600, 4256), (600, 2600, 8480)])
+def test_product_pieces(m, n, k):
+    a, w = operands(m, n, k, 7)
+    check_product(fp8.matmul_fp8(a, w, dtype=torch.float32), a, w)
+
+
 @pytest.mark.parametrize("m", [1, 3, 40, 200, 600])
 def test_product_strided_operands(m):
     """Operands and output as ranges of wider tensors; what lies beside the output stays."""

@@ -41,6 +41,10 @@ _raw_stream = torch._C._cuda_getCurrentRawStream
 _current_device = torch._C._cuda_getDevice
 _TYPE_IDS = {torch.float32: FORMATS["F32"].type_id, torch.float16: FORMATS["F16"].type_id,
              torch.bfloat16: FORMATS["BF16"].type_id}
+# Architectures (general.architecture of a GGUF file) whose feed-forward block is the one of
+# Fp8FeedForward.  Others hold tensors under the same names and compute something else with
+# them: Gemma takes tanh-GELU and, from its second version, a norm of the block's output.
+_GATED_SILU = ("llama", "mistral", "qwen2", "qwen3")
 
 
 class Fp8Rows(NamedTuple):
@@ -285,14 +289,24 @@ class Fp8FeedForward:
     @classmethod
     def from_gguf(cls, reader, layer: int, device=None) -> "Fp8FeedForward":
         """From a ``gguf.GGUFReader`` (or a path) by the tensors' GGUF names: ``blk.N.ffn_norm``,
-        ``ffn_gate``, ``ffn_up`` and ``ffn_down``; the epsilon from the file's metadata."""
+        ``ffn_gate``, ``ffn_up`` and ``ffn_down``; the epsilon from the file's metadata.  For files
+        of the architectures llama, mistral, qwen2 and qwen3; a file of another one, or a layer
+        with further feed-forward tensors (biases, a norm after the block, experts), computes
+        something else and is refused (``NotImplementedError``)."""
         if not hasattr(reader, "tensors"):
             from gguf import GGUFReader
             reader = GGUFReader(reader)
         from .gguf_conversion import _type_name, load_tensor
-        names = {t.name: t for t in reader.tensors}
-        norm, gate, up, down = (names[f"blk.{layer}.ffn_{part}.weight"] for part in ("norm", "gate", "up", "down"))
         arch = reader.fields["general.architecture"].contents()
+        if arch not in _GATED_SILU:
+            raise NotImplementedError(f"the feed-forward block of architecture {arch!r} is not known to be norm -> "
+                                      f"silu(gate) * up -> down (known: {', '.join(_GATED_SILU)})")
+        names = {t.name: t for t in reader.tensors}
+        parts = [f"blk.{layer}.ffn_{part}.weight" for part in ("norm", "gate", "up", "down")]
+        more = sorted(n for n in names if n.startswith((f"blk.{layer}.ffn_", f"blk.{layer}.post_ffw_")) and n not in parts)
+        if more:
+            raise NotImplementedError(f"layer {layer} has feed-forward tensors that this block does not take: {', '.join(more)}")
+        norm, gate, up, down = (names[part] for part in parts)
         eps = float(reader.fields[f"{arch}.attention.layer_norm_rms_epsilon"].contents())
         dev = torch.device("cuda" if device is None else device)
         rows, cols = (int(x) for x in gate.shape[::-1])

@@ -408,16 +408,13 @@ int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     CUtensorMap map{};
     if (boxes) {
         p.box_rows = static_cast<uint32_t>(hd == 0 ? 128 : std::min<int64_t>(hd, 128));
-        const EncodeTiled fn = encode_tiled();
-        if (fn == nullptr) return static_cast<int>(cudaErrorNotSupported);
         const cuuint64_t per = hd == 0 ? 1 : 2;
         const cuuint64_t dims[3] = {static_cast<cuuint64_t>(p.row_bytes / 4), per, static_cast<cuuint64_t>(p.rows) / per};
         const cuuint64_t strides[2] = {static_cast<cuuint64_t>(p.row_bytes), per * static_cast<cuuint64_t>(p.row_bytes)};
-        const cuuint32_t box[3] = {T::kPitch / 4, 1, p.box_rows}, step[3] = {1, 1, 1};
-        if (fn(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, const_cast<uint8_t*>(p.src), dims, strides, box, step,
-               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return static_cast<int>(cudaErrorInvalidValue);
+        const cuuint32_t box[3] = {T::kPitch / 4, 1, p.box_rows};
+        const int st = encode_map(&map, CU_TENSOR_MAP_DATA_TYPE_UINT32, 3, p.src, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_NONE,
+                                  CU_TENSOR_MAP_L2_PROMOTION_L2_128B);
+        if (st != 0) return st;
     }
     p.n_col_tiles = static_cast<uint32_t>((p.cols + 255) / 256);
     p.n_tiles = static_cast<uint32_t>((p.rows + 127) / 128 * p.n_col_tiles);

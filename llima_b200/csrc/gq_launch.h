@@ -51,19 +51,37 @@ int launch_early(void (*kern)(P...), unsigned grid, int threads, int smem, cudaS
     return static_cast<int>(cudaLaunchKernelEx(&cfg, kern, P(args)...));
 }
 
-using EncodeTiled = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                 CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+// A function of the loaded driver, or null
+template <class F>
+F driver_function(const char* name) {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult r;
+    if (cudaGetDriverEntryPoint(name, &f, cudaEnableDefault, &r) != cudaSuccess) f = nullptr;
+    return reinterpret_cast<F>(f);
+}
 
-// cuTensorMapEncodeTiled of the loaded driver, or null
-inline EncodeTiled encode_tiled() {
-    static const EncodeTiled fn = [] {
-        void* f = nullptr;
-        cudaDriverEntryPointQueryResult r;
-        if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &r) != cudaSuccess) f = nullptr;
-        return reinterpret_cast<EncodeTiled>(f);
-    }();
-    return fn;
+// Encodes a tensor map; the status as a runtime error code (the driver's have the same numbers).
+// The driver wants a context on the calling thread.  Launches bind the device's own, queries do
+// not, and a thread whose first CUDA work is one of these calls has none before this.
+inline int encode_map(CUtensorMap* map, CUtensorMapDataType type, cuuint32_t rank, const void* p, const cuuint64_t* dims,
+                      const cuuint64_t* strides, const cuuint32_t* box, CUtensorMapSwizzle swizzle, CUtensorMapL2promotion l2) {
+    using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    using GetContext = CUresult (*)(CUcontext*);
+    static const Encode encode = driver_function<Encode>("cuTensorMapEncodeTiled");
+    static const GetContext context = driver_function<GetContext>("cuCtxGetCurrent");
+    if (encode == nullptr || context == nullptr) return static_cast<int>(cudaErrorNotSupported);
+    CUcontext c = nullptr;
+    if (context(&c) != CUDA_SUCCESS || c == nullptr) {
+        int dev = 0;
+        cudaError_t e = cudaGetDevice(&dev);
+        if (e == cudaSuccess) e = cudaSetDevice(dev);
+        if (e != cudaSuccess) return static_cast<int>(e);
+    }
+    const cuuint32_t step[3] = {1, 1, 1};
+    return static_cast<int>(encode(map, type, rank, const_cast<void*>(p), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                                   swizzle, l2, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE));
 }
 
 }  // namespace gq

@@ -783,15 +783,12 @@ __global__ void __launch_bounds__(Wide<BN, T, PLAIN>::kThreads, 1)
 
 // (rows, k) bytes with a row stride, in boxes of box_rows x 128 bytes laid out in the
 // 128-byte swizzle
-bool tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {
-    const EncodeTiled fn = encode_tiled();
-    if (fn == nullptr) return false;
+int tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_t ld, int box_rows) {
     const cuuint64_t dims[2] = {static_cast<cuuint64_t>(k), static_cast<cuuint64_t>(rows)};
     const cuuint64_t strides[1] = {static_cast<cuuint64_t>(ld)};
-    const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)}, step[2] = {1, 1};
-    return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(p), dims, strides, box, step,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[2] = {kTileK, static_cast<cuuint32_t>(box_rows)};
+    return encode_map(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, p, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B,
+                      CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
 // How k is split: until about two CTAs per SM, with at least two 128-column blocks for each.
@@ -807,8 +804,9 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     using C = Narrow<BN, T>;
     auto kern = gq_matmul_narrow<BN, T>;
     CUtensorMap map_b, map_a;
-    if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, 128) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, BN))
-        return static_cast<int>(cudaErrorInvalidValue);
+    int st = tile_map(&map_b, p.b, p.n, p.k, p.ld_b, 128);
+    if (st == 0) st = tile_map(&map_a, p.a, p.m, p.k, p.ld_a, BN);
+    if (st != 0) return st;
     static std::atomic<uint64_t> allowed{0};
     cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
@@ -824,18 +822,16 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
     using C = Wide<BN, T, PLAIN>;
     auto kern = gq_matmul_wide<BN, T, PLAIN>;
     CUtensorMap map_b, map_a, map_out{};
-    if (!tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf) || !tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128))
-        return static_cast<int>(cudaErrorInvalidValue);
-    if (!PLAIN) {
+    int st = tile_map(&map_b, p.b, p.n, p.k, p.ld_b, C::kHalf);
+    if (st == 0) st = tile_map(&map_a, p.a, p.m, p.k, p.ld_a, 128);
+    if (!PLAIN && st == 0) {
         const cuuint64_t dims[2] = {static_cast<cuuint64_t>(p.n), static_cast<cuuint64_t>(p.m)};
         const cuuint64_t strides[1] = {static_cast<cuuint64_t>(p.ld_out) * sizeof(T)};
-        const cuuint32_t box[2] = {C::kBox / sizeof(T), 32}, step[2] = {1, 1};
-        if (encode_tiled()(&map_out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims,
-                           strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                           C::kBox == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
-                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-            return static_cast<int>(cudaErrorInvalidValue);
+        const cuuint32_t box[2] = {C::kBox / sizeof(T), 32};
+        st = encode_map(&map_out, sizeof(T) == 4 ? CU_TENSOR_MAP_DATA_TYPE_UINT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16, 2, p.out, dims, strides,
+                        box, C::kBox == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE);
     }
+    if (st != 0) return st;
     static std::atomic<uint64_t> allowed{0};
     const cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);

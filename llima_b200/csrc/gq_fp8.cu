@@ -403,7 +403,9 @@ int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     // boxes start on 128 bytes in shared memory: eight rows at least
     const bool boxes = p.row_bytes % 16 == 0 && (hd == 0 || (hd >= 8 && (128 % hd == 0 || hd % 128 == 0)));
     auto kern = boxes ? gq_fp8_weight_kernel<TYPE, true> : gq_fp8_weight_kernel<TYPE, false>;
-    const cudaError_t e = allow_smem(kern, T::kSmem, allowed[boxes]);
+    int sms = 0;
+    cudaError_t e = sm_count(sms);
+    if (e == cudaSuccess) e = allow_smem(kern, T::kSmem, allowed[boxes]);
     if (e != cudaSuccess) return static_cast<int>(e);
     CUtensorMap map{};
     if (boxes) {
@@ -419,7 +421,7 @@ int launch_weight(GqFp8Weight& p, cudaStream_t s) {
     p.n_col_tiles = static_cast<uint32_t>((p.cols + 255) / 256);
     p.n_tiles = static_cast<uint32_t>((p.rows + 127) / 128 * p.n_col_tiles);
     fast_div_params(p.n_col_tiles, p.ncol_mul, p.ncol_shift);
-    const uint32_t most = static_cast<uint32_t>(sm_count() * T::kPerSm);
+    const uint32_t most = static_cast<uint32_t>(sms * T::kPerSm);
     return launch_early(kern, std::min(p.n_tiles, most), T::kThreads, T::kSmem, s, 1, map, p);
 }
 template <class T>
@@ -742,8 +744,9 @@ template <class T, bool RESIDUAL, int NV>
 int launch_norm_rows(const GqFp8Rows& p, bool wide, cudaStream_t s) {
     auto kern = gq_fp8_norm_kernel<T, RESIDUAL, NV>;
     const int threads = static_cast<int>(((p.cols + 15) / 16 + 32 * NV - 1) / (32 * NV) * 32);
-    const int sms = sm_count();
-    int per = 0;
+    int sms = 0, per = 0;
+    const cudaError_t e = sm_count(sms);
+    if (e != cudaSuccess) return static_cast<int>(e);
     int64_t grid = p.rows;
     if (grid > sms) {
         cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per, kern, threads, 0);

@@ -9,11 +9,13 @@
 
 namespace gq {
 
-inline int sm_count() {
-    int dev = 0, sms = 0;
-    cudaGetDevice(&dev);
-    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    return sms;
+// SMs of the current device (at least 2)
+inline cudaError_t sm_count(int& sms) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess && sms < 2) e = cudaErrorInvalidDevice;
+    return e;
 }
 
 // The kernel's shared memory limit, raised once per device and kernel (`done`: a bit per device).

@@ -800,7 +800,7 @@ int narrow_split(const GqMatmul& p, int bn, int sms) {
 }
 
 template <int BN, class T>
-int launch_narrow(const GqMatmul& p, cudaStream_t s) {
+int launch_narrow(const GqMatmul& p, int sms, cudaStream_t s) {
     using C = Narrow<BN, T>;
     auto kern = gq_matmul_narrow<BN, T>;
     CUtensorMap map_b, map_a;
@@ -811,14 +811,14 @@ int launch_narrow(const GqMatmul& p, cudaStream_t s) {
     cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles = (p.m + BN - 1) / BN * ((p.n + 127) / 128);
-    const int split = narrow_split(p, BN, sm_count());
+    const int split = narrow_split(p, BN, sms);
     if (tiles * split > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     return launch_early(kern, static_cast<unsigned>(tiles * split), C::kThreads, C::kSmem, s, static_cast<unsigned>(split), map_b,
                         map_a, p, split);
 }
 
 template <int BN, class T, bool PLAIN>
-int launch_wide(const GqMatmul& p, cudaStream_t s) {
+int launch_wide(const GqMatmul& p, int sms, cudaStream_t s) {
     using C = Wide<BN, T, PLAIN>;
     auto kern = gq_matmul_wide<BN, T, PLAIN>;
     CUtensorMap map_b, map_a, map_out{};
@@ -839,7 +839,7 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
     if (tiles_m * tiles_n * p.kb > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     const bool use_raw = (reinterpret_cast<uintptr_t>(p.a_scales) & 15) == 0 && (reinterpret_cast<uintptr_t>(p.b_scales) & 15) == 0 &&
                          128 * p.ld_a_scales <= kRawA && BN / 128 * p.ld_b_scales + 32 <= kRawB;
-    const int64_t pairs = sm_count() / 2;
+    const int64_t pairs = sms / 2;
     const unsigned grid = static_cast<unsigned>(2 * (tiles_m * tiles_n < pairs ? tiles_m * tiles_n : pairs));
     // a band's tokens take about 37 MB (measured, held for a second: 8192 x 28672 x 4096 819 / 783 /
     // 756 / 756 us with bands of 4 / 8 / 16 / 32 tiles, 17 to 33 MB; 16384 x 8192 x 8192 857 / 852 / 866 /
@@ -861,8 +861,7 @@ int launch_wide(const GqMatmul& p, cudaStream_t s) {
 // 14.6; 768 x 4096 wide 256 16.8, wide 128 17.5; 160 x 4096, k = 14336 narrow 128 20.4, narrow 64
 // 24.0.  At most 1.11 times the best over 27 such shapes (512 x 4096, k = 512: 6.2 against 5.6).
 // Returns the narrow tile's tokens, or twice the wide tile's output channels.
-int choose(const GqMatmul& p, bool f32) {
-    const int sms = sm_count();
+int choose(const GqMatmul& p, bool f32, int sms) {
     const double hbm = static_cast<double>(p.m + p.n) * static_cast<double>(p.k) / 6.3e6;
     int best = 16;
     double least = 1e30;
@@ -905,14 +904,17 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     if (p.k == 0) {
         return launch_early(gq_matmul_bias<T>, 1024, 256, 0, s, 1, p);
     }
+    int sms = 0;
+    const cudaError_t e = sm_count(sms);
+    if (e != cudaSuccess) return static_cast<int>(e);
     const bool plain = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T))) % 16 != 0;
-    switch (choose(p, sizeof(T) == 4)) {
-        case 16: return launch_narrow<16, T>(p, s);
-        case 32: return launch_narrow<32, T>(p, s);
-        case 64: return launch_narrow<64, T>(p, s);
-        case 128: return launch_narrow<128, T>(p, s);
-        case 2 * 128: return plain ? launch_wide<128, T, true>(p, s) : launch_wide<128, T, false>(p, s);
-        default: return plain ? launch_wide<256, T, true>(p, s) : launch_wide<256, T, false>(p, s);
+    switch (choose(p, sizeof(T) == 4, sms)) {
+        case 16: return launch_narrow<16, T>(p, sms, s);
+        case 32: return launch_narrow<32, T>(p, sms, s);
+        case 64: return launch_narrow<64, T>(p, sms, s);
+        case 128: return launch_narrow<128, T>(p, sms, s);
+        case 2 * 128: return plain ? launch_wide<128, T, true>(p, sms, s) : launch_wide<128, T, false>(p, sms, s);
+        default: return plain ? launch_wide<256, T, true>(p, sms, s) : launch_wide<256, T, false>(p, sms, s);
     }
 }
 

@@ -243,8 +243,8 @@ GQ_API int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* 
  * extent do nothing, except that a product over k = 0 is the bias (or 0).
  *
  * gq_convert_fp8: a GGUF tensor (any type of gq_convert, perm_heads included; cols a
- * multiple of 32, rows at most 2^31 - 1) to tensor->codes, rows * cols e4m3 bytes, and scales, one per 128 x 128
- * block: (ceil(rows/128), ceil(cols/128)), row-major.  The values quantized are the f32
+ * multiple of 32, rows and cols at most 2^31 - 1) to tensor->codes, rows * cols e4m3 bytes, and
+ * scales, one per 128 x 128 block: (ceil(rows/128), ceil(cols/128)), row-major.  The values quantized are the f32
  * ones of GQ_OUT_F32.  tensor->scales, values and diag are not used.  src and codes 16-byte
  * aligned. */
 GQ_API int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream);

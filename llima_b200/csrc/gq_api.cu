@@ -519,7 +519,7 @@ int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream) {
     int64_t nv = 0, nu = 0;
     const int st = shape_check(t, &ti, &nv, &nu);
     if (st != GQ_OK) return st;
-    if (t.cols % 32 != 0 || t.rows > INT32_MAX) return GQ_ERR_SIZE;
+    if (rows_check(t.rows, t.cols) != GQ_OK) return GQ_ERR_SIZE;      // tile coordinates are 32-bit
     if (nv == 0) return GQ_OK;
     if (t.src == nullptr || t.codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
     if (!aligned(t.src, 16) || !aligned(t.codes, 16)) return GQ_ERR_ALIGN;

@@ -87,9 +87,8 @@ struct Narrow {
     static constexpr int kPieces = sizeof(T) < 4 || BN == 128 ? 1 : BN == 16 ? 4 : 3;      // accumulators
     static constexpr int kNeed = kPieces * BN + 8 * kSfSlots;
     static constexpr int kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
-    // CTAs that share an SM must find room in its 512 columns of tensor memory together, so
-    // that none waits for another's (in a cluster that could be a circle): shared memory is
-    // taken in the same proportion, 228 KB for 512 columns.
+    // CTAs that share an SM find room in its 512 columns of tensor memory together, so that none
+    // waits for another's: shared memory is taken in the same proportion, 228 KB for 512 columns.
     static constexpr int kLeast = kCols * 228 * 2 - 1024;
     static constexpr int kSmem = kUsed > kLeast ? kUsed : kLeast;
     static_assert(kRing >= BN * 128 * 4, "the sums fit the ring");
@@ -250,11 +249,21 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
             for (int j = 0; j < 16; ++j) sums[(c + j) * 128 + 32 * warp + lane] = __uint_as_float(v[j]);
         }
         tc::fence_before();
+        asm volatile("bar.arrive 1, 160;" ::: "memory");
     }
     if (!ok) atomicOr(&gq_matmul_errors, kErrWaitTimeout);
     __syncwarp();
-    if (split > 1) tc::cluster_sync();
+    if (split > 1) tc::cluster_arrive();
     else __syncthreads();
+    if (warp == 5) {
+        // The tensor memory goes back before this CTA waits for another one of its cluster, which
+        // may not have its own yet: a kernel of another stream that takes tensor memory by other
+        // proportions may hold it there, and wait here for this CTA's.
+        asm volatile("bar.sync 1, 160;" ::: "memory");
+        tc::fence_after();
+        tc::tmem_free<C::kCols>(tmem);
+    }
+    if (split > 1) tc::cluster_wait();
 
     T* const out = reinterpret_cast<T*>(p.out);
     const bool fours = ((reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T))) & (4 * sizeof(T) - 1)) == 0;
@@ -308,11 +317,6 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
     }
     // the partial sums stay until every CTA of the cluster has read them
     if (split > 1) tc::cluster_sync();
-    else __syncthreads();
-    if (warp == 5) {
-        tc::fence_after();
-        tc::tmem_free<C::kCols>(tmem);
-    }
 }
 
 // ---- wide products ----------------------------------------------------------------------------

@@ -70,7 +70,9 @@ __device__ __forceinline__ void init(uint32_t bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
 }
 
-// Every wait ends: false after kWaitLimitNs of global time without the phase completing.
+// Every wait ends: false after kWaitLimitNs of global time without the phase completing.  A whole
+// warp waits together and gets one answer: what follows in it (elect.sync, barriers) takes all 32
+// lanes on one way, also after a wait that gave up.
 // The waits order only what the asynchronous units do (tile loads, matrix instructions and
 // scale copies, tensor memory), never a thread's own reads of another CTA's writes, so none
 // acquires at cluster scope (measured: such a wait costs 600 to 900 cycles).
@@ -80,13 +82,13 @@ __device__ __forceinline__ bool try_wait(uint32_t bar, uint32_t parity) {
                  : "=r"(ok)
                  : "r"(bar), "r"(parity)
                  : "memory");
-    return ok != 0;
+    return __all_sync(0xffffffffu, ok != 0);
 }
 __device__ __forceinline__ bool wait(uint32_t bar, uint32_t parity) {
     if (try_wait(bar, parity)) return true;
     const uint64_t t0 = global_ns();
     while (!try_wait(bar, parity)) {
-        if (global_ns() - t0 > kWaitLimitNs) return false;
+        if (__any_sync(0xffffffffu, global_ns() - t0 > kWaitLimitNs)) return false;
     }
     return true;
 }

@@ -1,0 +1,22 @@
+"""The answer of the product's bounded wait is the warp's, not a lane's."""
+import ctypes
+import shutil
+import subprocess
+from pathlib import Path
+
+import pytest
+
+pytestmark = pytest.mark.gpu
+
+
+def test_a_warp_gets_one_answer(tmp_path):
+    from llima_b200.build import ARCH, CSRC
+    root = Path(__file__).resolve().parents[1]
+    so = tmp_path / "liblanes.so"
+    subprocess.run([shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc", *ARCH, "-O2", "-std=c++17", "-Xcompiler", "-fPIC", "-shared",
+                    f"-I{CSRC}", f"-I{root / 'include'}", "-o", str(so), str(root / "tests" / "cuda" / "tensor_wait_lanes.cu")],
+                   check=True, capture_output=True)
+    answers, elected = (ctypes.c_int * 64)(), (ctypes.c_int * 3)()
+    assert ctypes.CDLL(str(so)).run_lanes(answers, elected) == 0
+    assert list(answers) == [0] * 32 + [1] * 32
+    assert list(elected) == [1, 1, 3]

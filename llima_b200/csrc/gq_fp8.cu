@@ -148,6 +148,7 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
     using V = BlockView<TYPE>;
     using T = Fp8Tile<TYPE>;
     constexpr int NP = 32 / V::BV, NR = 2;                                  // blocks per 32 columns, rows per lane
+    constexpr uint32_t kGaveUp = 0xFFFFFFFFu;                               // above the bits of every finite magnitude
     constexpr bool kUnits16 = TYPE == GQ_TYPE_Q4_K || TYPE == GQ_TYPE_Q5_K;   // 9 and 11 times 16 bytes
     extern __shared__ __align__(128) uint8_t smem[];
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + T::kStages * T::kStageBytes);
@@ -213,13 +214,14 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
     uint8_t* const my_out = p.codes + static_cast<int64_t>(my_row) * p.cols + 32 * sub;
     const uint8_t* const my_smem = smem + my_row * T::kPitch;
     const uint32_t row_bytes16 = static_cast<uint32_t>(p.row_bytes) & 15u;
-    uint32_t n = 0;
     int s = 0;
-    uint32_t parity = 0, turn = 0;
-    for (uint32_t t = blockIdx.x; t < p.n_tiles; t += gridDim.x, ++n) {
+    uint32_t parity = 0, turn = 0, t = blockIdx.x;
+    for (; t < p.n_tiles; t += gridDim.x) {
+        // a wait that gave up ends the loop for all threads together, at this tile's barrier
         if (!mbar_wait(bars + s, parity)) {
             atomicOr(&gq_fp8_errors, kErrWaitTimeout);
-            break;
+            atomicMax(wmax + 2 * turn, kGaveUp);
+            atomicMax(wmax + 2 * turn + 1, kGaveUp);
         }
         const uint32_t tile_r = fast_div(t, p.ncol_mul, p.ncol_shift), tile_c = t - tile_r * p.n_col_tiles;
         const uint32_t row0 = tile_r * 128, rows = all_rows - row0, cols = all_cols - 256 * tile_c;    // left from here on
@@ -261,13 +263,15 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
             if (warp == 0) wmax[2 * turn + half] = 0;
         }
         __syncthreads();
+        const uint32_t block_amax_bits = *wm;
+        if (block_amax_bits == kGaveUp) break;
         // every thread is done with the stage
         if (t + T::kStages * gridDim.x < p.n_tiles) issue(t + T::kStages * gridDim.x, s);
         if (++s == T::kStages) {
             s = 0;
             parity ^= 1;
         }
-        const uint32_t byte = scale_byte(*wm);
+        const uint32_t byte = scale_byte(block_amax_bits);
         const float inv = inverse_scale(byte);
         if (warp == 0 && (lane & 27) == 0 && static_cast<uint32_t>(128 * half) < cols)
             p.scales[static_cast<int64_t>(tile_r) * p.scale_cols + 2 * tile_c + half] = static_cast<uint8_t>(byte);
@@ -289,11 +293,13 @@ __global__ void __launch_bounds__(Fp8Tile<TYPE>::kThreads, Fp8Tile<TYPE>::kPerSm
         }
     }
     // after a wait that gave up, nothing of this CTA stays in flight
-    if (static_cast<uint64_t>(blockIdx.x) + static_cast<uint64_t>(n) * gridDim.x < p.n_tiles)
-        for (int s = 0; s < T::kStages; ++s) {
-            const uint64_t t = blockIdx.x + static_cast<uint64_t>(n + s) * gridDim.x;
-            if (t < p.n_tiles) mbar_wait(bars + (n + s) % T::kStages, ((n + s) / T::kStages) & 1);
+    for (int i = 0; i < T::kStages && t < p.n_tiles; ++i, t += gridDim.x) {
+        mbar_wait(bars + s, parity);
+        if (++s == T::kStages) {
+            s = 0;
+            parity ^= 1;
         }
+    }
 }
 
 // ---- elements of the float types, eight at a time -----------------------------------------

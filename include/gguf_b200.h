@@ -126,10 +126,12 @@ GQ_API const char* gq_strerror(int status);
 /* CUDA error code (cudaError_t) behind the last GQ_ERR_CUDA of the calling thread. */
 GQ_API int gq_last_cuda_error(void);
 
-/* Sticky error flags of the conversion kernels on `device`, or-ed over every launch since
- * the last clear.  GQ_KERNEL_WAIT_TIMEOUT: a kernel waited about a second for a tile copy
- * that did not complete and stopped early, so that launch's outputs are incomplete.  The
- * flags live in device memory: read them once the work they should cover has finished.
+/* Sticky error flags of the conversion kernels and of the 8-bit float kernels
+ * (gq_convert_fp8, gq_matmul_fp8) on `device`, or-ed over every launch since the last clear.
+ * GQ_KERNEL_WAIT_TIMEOUT: a kernel waited about a second for a tile copy or a matrix
+ * instruction that did not complete and stopped early, so that launch's outputs are
+ * incomplete (a product's may hold partial sums).  The flags live in device memory: read
+ * them once the work they should cover has finished.
  * clear != 0 resets them.  No counterpart in the reference (whose numpy path cannot stall).
  * gq_convert_host and gq_convert_host_noalloc read and clear them themselves and fail with
  * GQ_ERR_CUDA (gq_last_cuda_error() = cudaErrorTimeout) when a flag was set. */

@@ -12,7 +12,8 @@ operators that feed them:
 * ``quantize_fp8``: rows, or silu(gate) * rows, quantized the same way;
 * ``matmul_fp8``: ``Fp8Rows`` times ``Fp8Weight``, for one token as for a long prompt;
 * ``Fp8Linear`` and ``Fp8FeedForward``: a projection, and a layer's gated feed-forward block,
-  from a GGUF file's tensors.
+  from a GGUF file's tensors;
+* ``check_kernels``: whether a kernel gave up waiting and left its result incomplete.
 
 Scales are ``float8_e8m0fnu``: 2^e with the smallest e >= -127 for which the block's largest
 finite magnitude is at most 448 * 2^e.  A value that is not finite becomes the NaN code.
@@ -33,7 +34,7 @@ from . import _native as N
 from .formats import FORMATS
 
 __all__ = ["Fp8Rows", "Fp8Weight", "convert_fp8_device", "fp8_from_gguf", "rms_norm_fp8", "quantize_fp8",
-           "matmul_fp8", "Fp8Linear", "Fp8FeedForward"]
+           "matmul_fp8", "check_kernels", "Fp8Linear", "Fp8FeedForward"]
 
 BLOCK = 128
 E4M3, E8M0 = torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -250,6 +251,23 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
           w_scales.data_ptr(), ld_sb, None if bias is None else _vector(bias, "bias", n, dev), m, n, k, _TYPE_IDS[dtype],
           out.data_ptr(), ld_o)
     return out
+
+
+def check_kernels(device=None) -> None:
+    """Waits for the work on ``device`` (a CUDA device, the current one by default) and raises
+    ``RuntimeError`` when one of the library's kernels there gave up a wait (for a tile copy, or
+    for the tensor cores, after a second) since the last call.  Such a kernel ends with its
+    result incomplete, and nothing else tells: a program that must not pass one on calls this
+    before it uses results, as seldom as it likes.  The record is cleared."""
+    torch.cuda.synchronize(device)
+    index = torch.device("cuda" if device is None else device).index if not isinstance(device, int) else device
+    if index is None:
+        index = torch.cuda.current_device()
+    flags = ctypes.c_uint32(0)
+    N.check(N.lib().gq_kernel_errors(index, 1, ctypes.byref(flags)), "gq_kernel_errors")
+    if flags.value:
+        raise RuntimeError(f"a kernel on cuda:{index} gave up waiting (flags {flags.value}): results since the last check may "
+                           "be incomplete")
 
 
 class Fp8Linear:

@@ -20,3 +20,13 @@ def test_a_warp_gets_one_answer(tmp_path):
     assert ctypes.CDLL(str(so)).run_lanes(answers, elected) == 0
     assert list(answers) == [0] * 32 + [1] * 32
     assert list(elected) == [1, 1, 3]
+
+
+def test_check_kernels_after_ordinary_work():
+    import torch
+    from llima_b200 import fp8
+    x = fp8.quantize_fp8(torch.randn(300, 512, device="cuda"))
+    w = fp8.convert_fp8_device("F32", torch.randn(512 * 512, device="cuda").view(torch.uint8), 512, 512)
+    fp8.matmul_fp8(x, w)
+    for device in (None, 0, "cuda", torch.device("cuda", 0)):
+        fp8.check_kernels(device)

@@ -364,8 +364,8 @@ __device__ __forceinline__ uint32_t raw_word(uint32_t a, bool words) {
 constexpr int kBatch = 4;
 
 // Outputs go out through shared memory, a few KB per warp, in the place of a stage of the ring
-// (measured: the ring loses nothing by it): as boxes of a tensor map where the rows start on 16
-// bytes, or (PLAIN) by the warp's own stores, a row's values side by side from neighbouring
+// (measured: the ring loses nothing by it): as boxes of a tensor map where the rows start and
+// end on 16 bytes, or (PLAIN) by the warp's own stores, a row's values side by side from neighbouring
 // lanes.  A lane that stores its own row directly touches 32 lines at a time (8192 x 28672 x 4096
 // 689 us against 649 without stores; 440 us for 6482 x 12260 x 320, whose rows start off 16 bytes).
 template <int BN, class T, bool PLAIN>
@@ -911,7 +911,10 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     int sms = 0;
     const cudaError_t e = sm_count(sms);
     if (e != cudaSuccess) return static_cast<int>(e);
-    const bool plain = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T))) % 16 != 0;
+    // Boxes end on 16 bytes, not on an element: where a row of the output does not, its last box would
+    // reach into what lies beside it.
+    const bool plain = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T)) |
+                        static_cast<uintptr_t>(p.n * sizeof(T))) % 16 != 0;
     switch (choose(p, sizeof(T) == 4, sms)) {
         case 16: return launch_narrow<16, T>(p, sms, s);
         case 32: return launch_narrow<32, T>(p, sms, s);

@@ -269,7 +269,8 @@ GQ_API int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const voi
                            int64_t ld_scales, void* stream);
 
 /* out (m, n) = a (m, k) * b (n, k)^T + bias (n, f32, or NULL), accumulated in f32 and rounded
- * once to dtype (GQ_TYPE_F32, F16 or BF16).  a: e4m3 with one scale per 1 x 128 block,
+ * once to dtype (GQ_TYPE_F32, F16 or BF16).  The tensor cores truncate as they accumulate; for
+ * f32 outputs they take sums of at most 6144 columns, which are added with rounding.  a: e4m3 with one scale per 1 x 128 block,
  * a_scales (m, ceil(k/128)); b: e4m3 with one scale per 128 x 128 block, b_scales
  * (ceil(n/128), ceil(k/128)).  k a multiple of 32; m, n and k at most 2^31 - 513; every row of a
  * and b starts on a 16-byte boundary, out and bias are aligned to their elements.  out must

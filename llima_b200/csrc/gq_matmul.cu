@@ -18,6 +18,7 @@
 
 #include <algorithm>
 
+#include "gq_choose.h"
 #include "gq_fp8.cuh"
 #include "gq_internal.h"
 #include "gq_launch.h"
@@ -70,11 +71,6 @@ __device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int64_t kb, i
 constexpr int kTileK = 128;
 constexpr int kSfSlots = 4;      // groups of four 128-column blocks whose scales are staged
 
-// The matrix instructions truncate as they add, so a sum's error grows with its length (1.7e-6 of
-// the result's norm over 112 blocks).  Where the output keeps f32, a sum is taken in pieces of
-// about kPiece blocks that are added in f32 with rounding; 16-bit outputs lose nothing by it.
-constexpr int kPiece = 32;
-
 template <int BN, class T>
 struct Narrow {
     static constexpr int kThreads = 192;
@@ -84,7 +80,7 @@ struct Narrow {
     static constexpr int kBars = 2 * kStages + 2 * kSfSlots + 1;
     static constexpr int kRing = kStages * kStageBytes;            // reused for the f32 sums
     static constexpr int kUsed = 1024 + kRing + kSfSlots * kSfBytes + 8 * kBars + 16;
-    static constexpr int kPieces = sizeof(T) < 4 || BN == 128 ? 1 : BN == 16 ? 4 : 3;      // accumulators
+    static constexpr int kPieces = narrow_pieces(BN, sizeof(T) == 4);      // accumulators
     static constexpr int kNeed = kPieces * BN + 8 * kSfSlots;
     static constexpr int kCols = kNeed <= 64 ? 64 : kNeed <= 128 ? 128 : 256;
     // CTAs that share an SM find room in its 512 columns of tensor memory together, so that none
@@ -795,14 +791,6 @@ int tile_map(CUtensorMap* map, const uint8_t* p, int64_t rows, int64_t k, int64_
                       CU_TENSOR_MAP_L2_PROMOTION_L2_256B);
 }
 
-// How k is split: until about two CTAs per SM, with at least two 128-column blocks for each.
-int narrow_split(const GqMatmul& p, int bn, int sms) {
-    const int64_t tiles = (p.m + bn - 1) / bn * ((p.n + 127) / 128);
-    int split = 1;
-    while (split < 8 && tiles * split <= sms && p.kb >= 4 * split) split *= 2;
-    return split;
-}
-
 template <int BN, class T>
 int launch_narrow(const GqMatmul& p, int sms, cudaStream_t s) {
     using C = Narrow<BN, T>;
@@ -815,7 +803,7 @@ int launch_narrow(const GqMatmul& p, int sms, cudaStream_t s) {
     cudaError_t e = allow_smem(kern, C::kSmem, allowed);
     if (e != cudaSuccess) return static_cast<int>(e);
     const int64_t tiles = (p.m + BN - 1) / BN * ((p.n + 127) / 128);
-    const int split = narrow_split(p, BN, sms);
+    const int split = narrow_split({p.m, p.n, p.k, p.kb}, BN, sizeof(T) == 4, sms);
     if (tiles * split > INT32_MAX) return static_cast<int>(cudaErrorInvalidValue);
     return launch_early(kern, static_cast<unsigned>(tiles * split), C::kThreads, C::kSmem, s, static_cast<unsigned>(split), map_b,
                         map_a, p, split);
@@ -853,44 +841,6 @@ int launch_wide(const GqMatmul& p, int sms, cudaStream_t s) {
     return launch_early(kern, grid, C::kThreads, C::kSmem, s, 2, map_a, map_b, map_out, p, order, use_raw);
 }
 
-// Which kernel and tile: the least estimated time (us).  A narrow tile costs what its operands
-// take through an SM's read path (133 KB a us), the busiest SM counts, and no less than reading
-// the operands from HBM (6.3 MB a us); set-up and the sums' way out grow with the tile and come
-// again with every round of CTAs.  A wide
-// one costs its tiles (0.287 us per 256 x 256 x 128 on a pair, the matrix instructions' rate; 0.19 per
-// 256 x 128 x 128, where the way from the L2 bounds it: 24 KB per SM) and a drain, in rounds over
-// the pairs.  Measured against it (us, k = 4096 unless said; the best and the runner-up): 64 x 28672
-// narrow 64 23.2, narrow 128 24.7; 96 x 28672 narrow 128 26.1, wide 256 30.3; 160 x 28672 wide 256
-// 31.5, wide 128 33.8; 128 x 4096 narrow 64 9.0, wide 128 11.0; 512 x 4096 wide 128 12.0, narrow 64
-// 14.6; 768 x 4096 wide 256 16.8, wide 128 17.5; 160 x 4096, k = 14336 narrow 128 20.4, narrow 64
-// 24.0.  At most 1.11 times the best over 27 such shapes (512 x 4096, k = 512: 6.2 against 5.6).
-// Returns the narrow tile's tokens, or twice the wide tile's output channels.
-int choose(const GqMatmul& p, bool f32, int sms) {
-    const double hbm = static_cast<double>(p.m + p.n) * static_cast<double>(p.k) / 6.3e6;
-    int best = 16;
-    double least = 1e30;
-    const auto take = [&](int what, double us) {
-        if (us < least) {
-            least = us;
-            best = what;
-        }
-    };
-    for (int bn : {16, 32, 64, 128}) {
-        const int split = narrow_split(p, bn, sms);
-        if (f32 && bn == 128 && p.kb > 3 * kPiece / 2 * split) continue;      // a sum in one piece (see kPiece)
-        const int64_t ctas = (p.m + bn - 1) / bn * ((p.n + 127) / 128) * split;
-        const double bytes = static_cast<double>((ctas + sms - 1) / sms) * static_cast<double>((p.kb + split - 1) / split) * (128 + bn) * 128;
-        const double rounds = static_cast<double>((ctas + 2 * sms - 1) / (2 * sms));      // two CTAs on an SM
-        take(bn, rounds * (3.0 + 0.032 * bn) + (split > 1 ? 1.0 : 0.0) + std::max(bytes / 133e3, hbm));
-    }
-    for (int bn : {128, 256}) {
-        const int64_t tiles = (p.m + 255) / 256 * ((p.n + bn - 1) / bn), pairs = sms / 2;
-        const double each = bn == 128 ? 0.19 * static_cast<double>(p.kb) + 1.7 : 0.287 * static_cast<double>(p.kb) + 2.8;
-        take(2 * bn, 5.0 + std::max(static_cast<double>((tiles + pairs - 1) / pairs) * each, hbm));
-    }
-    return best;
-}
-
 // out = bias (or 0): a product over no columns
 template <class T>
 __global__ void gq_matmul_bias(const GqMatmul p) {
@@ -915,7 +865,7 @@ int launch_t(const GqMatmul& p, cudaStream_t s) {
     // reach into what lies beside it.
     const bool plain = (reinterpret_cast<uintptr_t>(p.out) | static_cast<uintptr_t>(p.ld_out * sizeof(T)) |
                         static_cast<uintptr_t>(p.n * sizeof(T))) % 16 != 0;
-    switch (choose(p, sizeof(T) == 4, sms)) {
+    switch (choose({p.m, p.n, p.k, p.kb}, sizeof(T) == 4, sms)) {
         case 16: return launch_narrow<16, T>(p, sms, s);
         case 32: return launch_narrow<32, T>(p, sms, s);
         case 64: return launch_narrow<64, T>(p, sms, s);

@@ -225,7 +225,9 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
                out: torch.Tensor | None = None) -> torch.Tensor:
     """a (m, k) times w (n, k) transposed, plus ``bias`` (n, float32): (m, n) of ``dtype``
     (bfloat16, float16 or float32; that of ``out`` when given), accumulated in float32 and
-    rounded once.  ``out`` must not overlap the operands."""
+    rounded once.  The tensor cores truncate as they accumulate; for float32 results they take
+    sums of at most 6144 columns, which are added with rounding.  ``out`` must not overlap the
+    operands."""
     codes, scales = a
     w_codes, w_scales = w
     dev = _device_of(codes, "a.codes")

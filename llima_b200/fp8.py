@@ -20,7 +20,8 @@ finite magnitude is at most 448 * 2^e.  A value that is not finite becomes the N
 Row counts are free; column counts are multiples of 32, as every quantized GGUF row's are.
 
 Work is enqueued on the current stream of the operands' device, whichever device is
-current, and no call waits for it.
+current, and no call waits for it.  There are no gradients: outside ``torch.no_grad()`` an operand
+that requires one is refused.
 """
 from __future__ import annotations
 
@@ -73,6 +74,22 @@ def _call(name: str, device: int, *args) -> None:
             status = getattr(N.lib(), name)(*args, _raw_stream(device))
     if status:
         N.check(status, name)
+
+
+def _no_backward(*tensors: torch.Tensor | None) -> None:
+    """These operators have no backward pass: an operand that a gradient is asked for is refused
+    rather than detached in silence.  (Callers look at ``requires_grad`` themselves first: a call
+    costs half a microsecond.)"""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("no gradients through the 8-bit float operators: detach the operand, or call under torch.no_grad()")
+
+
+def _written(*tensors: torch.Tensor) -> None:
+    """Tells autograd that these tensors of the caller's were written, so that a backward pass that
+    saved what was there before fails instead of using what is there now."""
+    for t in tensors:
+        if not t.is_inference():
+            torch.autograd.graph.increment_version(t)
 
 
 def _matrix(t: torch.Tensor, name: str, dtype, device: int, rows: int | None = None, cols: int | None = None) -> int:
@@ -147,11 +164,13 @@ def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads:
         raise TypeError("src must be a contiguous CUDA uint8 tensor of GGUF bytes")
     dev = src.get_device()
     shape = ((rows + BLOCK - 1) // BLOCK, (cols + BLOCK - 1) // BLOCK)
+    given = out
     if out is None:
         if rows < 0 or cols < 0:
             raise ValueError(f"negative shape ({rows}, {cols})")
         out = Fp8Weight(_new(rows, cols, E4M3, src.device), _new(*shape, E8M0, src.device))
     else:
+        _no_backward(*out)
         _matrix(out.codes, "out.codes", E4M3, dev, rows, cols)
         _matrix(out.scales, "out.scales", E8M0, dev, *shape)
         if not out.codes.is_contiguous() or not out.scales.is_contiguous():
@@ -159,6 +178,8 @@ def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads:
     t = N.Tensor(type=f.type_id, perm_heads=heads, rows=rows, cols=cols, src=src.data_ptr(), src_bytes=src.numel(),
                  codes=out.codes.data_ptr())
     _call("gq_convert_fp8", dev, ctypes.byref(t), out.scales.data_ptr())
+    if given is not None:
+        _written(*out)
     return out
 
 
@@ -183,12 +204,16 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
     h / sqrt(mean(h^2) + eps) * weight, weight float32 (cols).  With ``residual`` (of x's
     type and shape), h = x + residual rounded to that type and (``Fp8Rows``, h) is returned;
     ``sum_out`` receives h and may be ``residual`` or ``x`` itself."""
+    if x.requires_grad or weight.requires_grad or residual is not None and residual.requires_grad or \
+            sum_out is not None and sum_out.requires_grad or out is not None:
+        _no_backward(x, weight, residual, sum_out, *(out or ()))
     ld_x = _float_rows(x, "x")
     rows, cols = x.shape
     dev = x.get_device()
     w = _vector(weight, "weight", cols, dev)
     ld_r = ld_s = 0
     r = s = None
+    given = sum_out
     if residual is not None:
         ld_r = _matrix(residual, "residual", x.dtype, dev, rows, cols)
         if sum_out is None:
@@ -201,6 +226,10 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5, resid
     codes, ld_c, scales, ld_sc = _rows_out(x, dev, out)
     _call("gq_rms_norm_fp8", dev, _TYPE_IDS[x.dtype], x.data_ptr(), ld_x, r, ld_r, w, eps, rows, cols, s, ld_s,
           codes.data_ptr(), ld_c, scales.data_ptr(), ld_sc)
+    if out is not None:
+        _written(*out)
+    if given is not None:
+        _written(given)
     q = Fp8Rows(codes, scales)
     return q if residual is None else (q, sum_out)
 
@@ -209,6 +238,8 @@ def quantize_fp8(x: torch.Tensor, gate: torch.Tensor | None = None, out: Fp8Rows
     """Rows of ``x`` (rows, cols), or silu(gate) * x with ``gate`` of x's type and shape, as
     ``Fp8Rows``.  Both may be column ranges of one wider tensor, as a fused gate and up
     product leaves them."""
+    if x.requires_grad or gate is not None and gate.requires_grad or out is not None:
+        _no_backward(x, gate, *(out or ()))
     ld_x = _float_rows(x, "x")
     rows, cols = x.shape
     dev = x.get_device()
@@ -218,6 +249,8 @@ def quantize_fp8(x: torch.Tensor, gate: torch.Tensor | None = None, out: Fp8Rows
     codes, ld_c, scales, ld_sc = _rows_out(x, dev, out)
     _call("gq_quantize_fp8", dev, _TYPE_IDS[x.dtype], x.data_ptr(), ld_x, g, ld_g, rows, cols, codes.data_ptr(), ld_c,
           scales.data_ptr(), ld_sc)
+    if out is not None:
+        _written(*out)
     return Fp8Rows(codes, scales)
 
 
@@ -230,6 +263,9 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     operands."""
     codes, scales = a
     w_codes, w_scales = w
+    if codes.requires_grad or w_codes.requires_grad or scales.requires_grad or w_scales.requires_grad or \
+            bias is not None and bias.requires_grad or out is not None and out.requires_grad:
+        _no_backward(codes, scales, w_codes, w_scales, bias, out)
     dev = _device_of(codes, "a.codes")
     ld_a = _matrix(codes, "a.codes", E4M3, dev)
     m, k = codes.shape
@@ -240,6 +276,7 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     ld_b = _matrix(w_codes, "w.codes", E4M3, dev, None, k)
     n = w_codes.shape[0]
     ld_sb = _matrix(w_scales, "w.scales", E8M0, dev, (n + 127) >> 7, blocks)
+    given = out
     if out is None:
         if dtype not in _TYPE_IDS:
             raise TypeError(f"dtype must be float32, float16 or bfloat16, not {dtype}")
@@ -252,6 +289,8 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     _call("gq_matmul_fp8", dev, codes.data_ptr(), ld_a, scales.data_ptr(), ld_sa, w_codes.data_ptr(), ld_b,
           w_scales.data_ptr(), ld_sb, None if bias is None else _vector(bias, "bias", n, dev), m, n, k, _TYPE_IDS[dtype],
           out.data_ptr(), ld_o)
+    if given is not None:
+        _written(out)
     return out
 
 

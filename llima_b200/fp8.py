@@ -154,12 +154,18 @@ def _rows_out(x: torch.Tensor, device: int, out: Fp8Rows | None):
             scales, _matrix(scales, "out.scales", E8M0, device, rows, blocks))
 
 
+def _known(fmt: str) -> str:
+    if fmt not in FORMATS:
+        raise NotImplementedError(f"GGML type {fmt} is not handled by the B200 GGUF path")
+    return fmt
+
+
 def convert_fp8_device(fmt: str, src: torch.Tensor, rows: int, cols: int, heads: int = 0,
                        out: Fp8Weight | None = None) -> Fp8Weight:
     """GGUF bytes already on the GPU (uint8, 16-byte aligned) -> ``Fp8Weight``.  The values
     quantized are those of the f32 conversion, bit for bit; heads > 0 applies the llama q/k
     row permutation (``GgufModel._permute_qk_proj``, gguf_conversion.py:314-332)."""
-    f = FORMATS[fmt]
+    f = FORMATS[_known(fmt)]
     if src.dtype != torch.uint8 or not src.is_cuda or not src.is_contiguous():
         raise TypeError("src must be a contiguous CUDA uint8 tensor of GGUF bytes")
     dev = src.get_device()
@@ -187,9 +193,7 @@ def fp8_from_gguf(gguf_tensor, heads: int = 0, device=None) -> Fp8Weight:
     """``Fp8Weight`` of one reader tensor (rows = output channels).  ``device``: a CUDA
     device, the current one by default."""
     from .gguf_conversion import _type_name
-    fmt = _type_name(gguf_tensor.tensor_type)
-    if fmt not in FORMATS:
-        raise NotImplementedError(f"GGML type {fmt} is not handled by the B200 GGUF path")
+    fmt = _known(_type_name(gguf_tensor.tensor_type))
     shape = tuple(int(x) for x in gguf_tensor.shape[::-1])
     if len(shape) != 2:
         raise ValueError(f"{gguf_tensor.name}: a weight has two dimensions, not {len(shape)}")

@@ -26,6 +26,7 @@ that requires one is refused.
 from __future__ import annotations
 
 import ctypes
+import math
 from typing import NamedTuple
 
 import numpy as np
@@ -326,6 +327,9 @@ class Fp8Linear:
     def from_gguf(cls, gguf_tensor, bias_tensor=None, heads: int = 0, device=None) -> "Fp8Linear":
         """From a reader's weight tensor and, where the model has one, its bias tensor;
         heads > 0 applies the llama q/k row permutation to both."""
+        if bias_tensor is not None and math.prod(int(x) for x in bias_tensor.shape) != int(gguf_tensor.shape[-1]):
+            raise ValueError(f"{bias_tensor.name} has shape {tuple(bias_tensor.shape)}: {gguf_tensor.name} has "
+                             f"{int(gguf_tensor.shape[-1])} output channels")
         weight = fp8_from_gguf(gguf_tensor, heads, device)
         bias = None
         if bias_tensor is not None:
@@ -372,9 +376,14 @@ class Fp8FeedForward:
         norm, gate, up, down = (names[part] for part in parts)
         eps = float(reader.fields[f"{arch}.attention.layer_norm_rms_epsilon"].contents())
         dev = torch.device("cuda" if device is None else device)
-        rows, cols = (int(x) for x in gate.shape[::-1])
-        if tuple(up.shape) != tuple(gate.shape):
-            raise ValueError(f"gate and up weights differ in shape: {tuple(gate.shape)}, {tuple(up.shape)}")
+        shapes = [tuple(int(x) for x in t.shape[::-1]) for t in (gate, up, down, norm)]
+        if len(shapes[0]) != 2:
+            raise ValueError(f"{gate.name}: a weight has two dimensions, not {len(shapes[0])}")
+        rows, cols = shapes[0]
+        if shapes != [(rows, cols), (rows, cols), (cols, rows), (cols,)]:
+            raise ValueError("the shapes of gate, up, down and norm do not belong together: " + ", ".join(map(str, shapes)))
+        for t in (gate, up, down):
+            _known(_type_name(t.tensor_type))
         if rows % BLOCK:
             raise ValueError(f"{rows} feed-forward channels: a multiple of {BLOCK} is needed to keep the gate and up "
                              "weights in one tensor")

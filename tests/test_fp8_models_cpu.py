@@ -65,3 +65,27 @@ def test_layers_with_more_tensors(tmp_path, name, no_gpu):
     path = write_file(tmp_path / "m.gguf", extra=[f"blk.0.{name}"])
     with pytest.raises(NotImplementedError, match=name):
         fp8.Fp8FeedForward.from_gguf(path, 0, device="cpu")
+
+
+@pytest.mark.parametrize("change", [{"shapes": ((256, 128), (384, 128), (128, 256))}, {"shapes": ((256, 128), (256, 160), (128, 256))},
+                                    {"shapes": ((256, 128), (256, 128), (128, 288))}, {"shapes": ((256, 128), (256, 128), (160, 256))},
+                                    {"norm": 160}, {"shapes": ((256, 160), (256, 160), (160, 256))}])
+def test_shapes_that_do_not_belong_together(tmp_path, change, no_gpu):
+    path = write_file(tmp_path / "m.gguf", **change)
+    with pytest.raises(ValueError, match="do not belong together"):
+        fp8.Fp8FeedForward.from_gguf(path, 0, device="cpu")
+
+
+def test_feed_forward_channels_off_the_block(tmp_path, no_gpu):
+    path = write_file(tmp_path / "m.gguf", shapes=((320, 128), (320, 128), (128, 320)))
+    with pytest.raises(ValueError, match="multiple of 128"):
+        fp8.Fp8FeedForward.from_gguf(path, 0, device="cpu")
+
+
+def test_a_bias_of_another_length(tmp_path, no_gpu):
+    path = write_file(tmp_path / "m.gguf", extra=["blk.0.attn_q.bias"])
+    t = {t.name: t for t in gguf.GGUFReader(path).tensors}
+    with pytest.raises(ValueError, match="256 output channels"):
+        fp8.Fp8Linear.from_gguf(t["blk.0.ffn_gate.weight"], t["blk.0.attn_q.bias"], device="cpu")
+    with pytest.raises(Reached):
+        fp8.Fp8Linear.from_gguf(t["blk.0.ffn_down.weight"], t["blk.0.attn_q.bias"], device="cpu")

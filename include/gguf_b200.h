@@ -242,7 +242,9 @@ GQ_API int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* 
  * accelerator (ModelGraph.linear, sima_lmm/model/model_graph.py:351-403): these four run a
  * GGUF file's projections on the GPU itself.  Device pointers of the current device; all
  * strides are in elements, and the elements of a row are consecutive.  Shapes with a zero
- * extent do nothing, except that a product over k = 0 is the bias (or 0).
+ * extent do nothing, except that a product over k = 0 is the bias (or 0).  Outputs share no
+ * byte with the inputs or with one another, except where stated; calls in which they do are
+ * refused (GQ_ERR_ARG).
  *
  * gq_convert_fp8: a GGUF tensor (any type of gq_convert, perm_heads included; cols a
  * multiple of 32, rows and cols at most 2^31 - 1) to tensor->codes, rows * cols e4m3 bytes, and
@@ -273,8 +275,7 @@ GQ_API int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const voi
  * f32 outputs they take sums of at most 6144 columns, which are added with rounding.  a: e4m3 with one scale per 1 x 128 block,
  * a_scales (m, ceil(k/128)); b: e4m3 with one scale per 128 x 128 block, b_scales
  * (ceil(n/128), ceil(k/128)).  k a multiple of 32; m, n and k at most 2^31 - 513; every row of a
- * and b starts on a 16-byte boundary, out and bias are aligned to their elements.  out must
- * not overlap the inputs. */
+ * and b starts on a 16-byte boundary, out and bias are aligned to their elements. */
 GQ_API int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64_t ld_a_scales,
                          const uint8_t* b, int64_t ld_b, const uint8_t* b_scales, int64_t ld_b_scales,
                          const float* bias, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <cerrno>
 #include <deque>
+#include <initializer_list>
 #include <map>
 #include <unordered_map>
 #include <condition_variable>
@@ -149,6 +150,40 @@ int rows_check(int64_t rows, int64_t cols) {
 // every row starts on a 16-byte boundary
 bool rows_aligned(const void* p, int64_t ld, int64_t rows, int elem_bytes) {
     return aligned(p, 16) && (rows <= 1 || ld % (16 / elem_bytes) == 0);
+}
+
+// Rows of `width` bytes, `stride` bytes apart
+struct Rows {
+    const void* p;
+    int64_t rows, stride, width;
+};
+
+// Whether two of them share a byte.  Where strides differ and neither has one row only, ranges that
+// meet count as sharing.
+bool overlap(const Rows& x, const Rows& y) {
+    if (x.p == nullptr || y.p == nullptr || x.rows <= 0 || y.rows <= 0 || x.width <= 0 || y.width <= 0) return false;
+    const int64_t d = static_cast<int64_t>(reinterpret_cast<uintptr_t>(y.p) - reinterpret_cast<uintptr_t>(x.p));
+    using Wide = __int128;       // rows times strides
+    if (d >= Wide(x.rows - 1) * x.stride + x.width || -Wide(d) >= Wide(y.rows - 1) * y.stride + y.width) return false;
+    if (x.rows == 1 && y.rows == 1) return true;
+    const int64_t s = x.rows == 1 ? y.stride : x.stride;
+    if (y.rows > 1 && y.stride != s) return true;
+    // row j of y begins d + (j - i) s bytes after row i of x: the first of them past -y.width
+    const Wide t = -Wide(y.width) - d;
+    const Wide first = (t >= 0 ? t / s : -((-t + s - 1) / s)) + 1, m = std::max<Wide>(first, 1 - x.rows);
+    return m <= y.rows - 1 && d + m * s < x.width;
+}
+bool same(const Rows& x, const Rows& y) { return x.p == y.p && x.width == y.width && (x.rows <= 1 || x.stride == y.stride); }
+
+// Whether an output shares a byte with an input or with another output.
+bool overlap_any(std::initializer_list<Rows> outputs, std::initializer_list<Rows> inputs) {
+    for (const Rows* o = outputs.begin(); o != outputs.end(); ++o) {
+        for (const Rows& i : inputs)
+            if (overlap(*o, i)) return true;
+        for (const Rows* other = o + 1; other != outputs.end(); ++other)
+            if (overlap(*o, *other)) return true;
+    }
+    return false;
 }
 
 gq::GqDesc make_desc(const gq_tensor_t& t, const TypeInfo& ti, int64_t n_units) {
@@ -533,6 +568,8 @@ int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream) {
     p.src_bytes = nu * ti.unit_bytes;
     p.scale_cols = (t.cols + 127) / 128;
     if ((t.rows + 127) / 128 > INT32_MAX / p.scale_cols) return GQ_ERR_SIZE;
+    if (overlap_any({{t.codes, 1, 0, nv}, {scales, 1, 0, (t.rows + 127) / 128 * p.scale_cols}}, {{t.src, 1, 0, p.src_bytes}}))
+        return GQ_ERR_ARG;
     if (t.perm_heads > 0) p.head_dim = static_cast<uint32_t>(t.rows / t.perm_heads);
     return cuda_status(gq::launch_fp8_weight(t.type, p, stream));
 }
@@ -546,12 +583,18 @@ int gq_rms_norm_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* resi
     if (st != GQ_OK) return st;
     if (ld_x < cols || ld_codes < cols || ld_scales < (cols + 127) / 128) return GQ_ERR_SIZE;
     if (residual != nullptr && (ld_residual < cols || ld_sum < cols)) return GQ_ERR_SIZE;
+    if (std::max({ld_x, ld_codes, ld_scales, residual != nullptr ? std::max(ld_residual, ld_sum) : 0}) > kMaxStride) return GQ_ERR_SIZE;
     if (rows == 0 || cols == 0) return GQ_OK;
     if (x == nullptr || weight == nullptr || codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
     if (residual != nullptr && sum == nullptr) return GQ_ERR_NULL;
     if (!rows_aligned(x, ld_x, rows, es) || !rows_aligned(codes, ld_codes, rows, 1) || !aligned(weight, 16)) return GQ_ERR_ALIGN;
     if (residual != nullptr && (!rows_aligned(residual, ld_residual, rows, es) || !rows_aligned(sum, ld_sum, rows, es)))
         return GQ_ERR_ALIGN;
+    const Rows rx{x, rows, ld_x * es, cols * es}, rr{residual, rows, ld_residual * es, cols * es}, rw{weight, 1, 0, cols * 4};
+    const Rows rs{residual != nullptr ? sum : nullptr, rows, ld_sum * es, cols * es};
+    const Rows rc{codes, rows, ld_codes, cols}, rb{scales, rows, ld_scales, (cols + 127) / 128};
+    if (overlap_any({rc, rb}, {rx, rr, rw, rs}) || overlap(rs, rw)) return GQ_ERR_ARG;
+    if ((!same(rs, rx) && overlap(rs, rx)) || (!same(rs, rr) && overlap(rs, rr))) return GQ_ERR_ARG;
     gq::GqFp8Rows p{};
     p.x = static_cast<const uint8_t*>(x);
     p.residual = static_cast<const uint8_t*>(residual);
@@ -579,10 +622,14 @@ int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* gate
     if (st != GQ_OK) return st;
     if (ld_x < cols || ld_codes < cols || ld_scales < (cols + 127) / 128) return GQ_ERR_SIZE;
     if (gate != nullptr && ld_gate < cols) return GQ_ERR_SIZE;
+    if (std::max({ld_x, ld_codes, ld_scales, gate != nullptr ? ld_gate : 0}) > kMaxStride) return GQ_ERR_SIZE;
     if (rows == 0 || cols == 0) return GQ_OK;
     if (x == nullptr || codes == nullptr || scales == nullptr) return GQ_ERR_NULL;
     if (!rows_aligned(x, ld_x, rows, es) || !rows_aligned(codes, ld_codes, rows, 1)) return GQ_ERR_ALIGN;
     if (gate != nullptr && !rows_aligned(gate, ld_gate, rows, es)) return GQ_ERR_ALIGN;
+    if (overlap_any({{codes, rows, ld_codes, cols}, {scales, rows, ld_scales, (cols + 127) / 128}},
+                    {{x, rows, ld_x * es, cols * es}, {gate, rows, ld_gate * es, cols * es}}))
+        return GQ_ERR_ARG;
     gq::GqFp8Rows p{};
     p.x = static_cast<const uint8_t*>(x);
     p.gate = static_cast<const uint8_t*>(gate);
@@ -614,6 +661,9 @@ int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64
     if (k != 0 && (a == nullptr || b == nullptr || a_scales == nullptr || b_scales == nullptr)) return GQ_ERR_NULL;
     if (!aligned(out, es) || !aligned(bias, 4)) return GQ_ERR_ALIGN;
     if (k != 0 && (!rows_aligned(a, ld_a, m, 1) || !rows_aligned(b, ld_b, n, 1))) return GQ_ERR_ALIGN;
+    if (overlap_any({{out, m, ld_out * es, n * es}}, {{a, m, ld_a, k}, {a_scales, m, ld_a_scales, kb}, {b, n, ld_b, k},
+                                                      {b_scales, (n + 127) / 128, ld_b_scales, kb}, {bias, 1, 0, n * 4}}))
+        return GQ_ERR_ARG;
     gq::GqMatmul p{};
     p.a = a;
     p.a_scales = a_scales;

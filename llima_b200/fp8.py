@@ -21,7 +21,8 @@ Row counts are free; column counts are multiples of 32, as every quantized GGUF 
 
 Work is enqueued on the current stream of the operands' device, whichever device is
 current, and no call waits for it.  There are no gradients: outside ``torch.no_grad()`` an operand
-that requires one is refused.
+that requires one is refused.  A tensor given as ``out`` or ``sum_out`` shares no memory with
+another operand except where stated (refused as well).
 """
 from __future__ import annotations
 
@@ -264,8 +265,7 @@ def matmul_fp8(a: Fp8Rows, w: Fp8Weight, bias: torch.Tensor | None = None, dtype
     """a (m, k) times w (n, k) transposed, plus ``bias`` (n, float32): (m, n) of ``dtype``
     (bfloat16, float16 or float32; that of ``out`` when given), accumulated in float32 and
     rounded once.  The tensor cores truncate as they accumulate; for float32 results they take
-    sums of at most 6144 columns, which are added with rounding.  ``out`` must not overlap the
-    operands."""
+    sums of at most 6144 columns, which are added with rounding."""
     codes, scales = a
     w_codes, w_scales = w
     if codes.requires_grad or w_codes.requires_grad or scales.requires_grad or w_scales.requires_grad or \

@@ -27,7 +27,7 @@ def calls():
     yield "feed forward", lambda: fp8.Fp8FeedForward(w, weight, weight)(leaf, x)
 
 
-@pytest.mark.parametrize("name,call", calls(), ids=lambda v: v if isinstance(v, str) else "")
+@pytest.mark.parametrize("name,call", list(calls()), ids=lambda v: v if isinstance(v, str) else "")
 def test_gradients_are_refused(name, call):
     with pytest.raises(RuntimeError, match="no gradients"):
         call()

@@ -483,8 +483,22 @@ struct Raw16 {
     // value pair i of 8
     __device__ __forceinline__ float2 get(int i) const {
         if constexpr (std::is_same<T, F32>::value) return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
-        else if constexpr (std::is_same<T, F16>::value) return __half22float2(u32_as_h2(w[i]));
-        else return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xFFFF0000u));
+        else return widen(w[i]);
+    }
+    static __device__ __forceinline__ float2 widen(uint32_t v) {
+        if constexpr (std::is_same<T, F16>::value) return __half22float2(u32_as_h2(v));
+        else return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xFFFF0000u));
+    }
+    // one pair on its own
+    static __device__ __forceinline__ float2 load2(const uint8_t* p) {
+        uint32_t a, b;
+        if constexpr (std::is_same<T, F32>::value) {
+            asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(a), "=r"(b) : "l"(p));
+            return make_float2(__uint_as_float(a), __uint_as_float(b));
+        } else {
+            asm volatile("ld.global.b32 %0, [%1];" : "=r"(a) : "l"(p));
+            return widen(a);
+        }
     }
     // rounds to the type
     __device__ __forceinline__ void set(int i, float2 v) {
@@ -539,16 +553,28 @@ __device__ __forceinline__ uint4 quantize_block(float2 (&y)[8], uint32_t& byte) 
     return make_uint4(c[0], c[1], c[2], c[3]);
 }
 
-// silu(g) * x of two values, with u = exp(-|g| / 2): g / (1 + u^2) * x, for g < 0 times u^2, one u
-// to each factor.  Nothing overflows, and no factor leaves the normal range before |g| = 174, where
-// the formula's own exponential overflows at g = -88.7 and its quotient leaves the normal range at
-// -87.3.  Relative error: u's exponent is off by 1.25 * 2^-24 of itself (the product and the
-// constant), which u^2 shows as |g| 2^-23.7 (in the sum of s it cancels rather than adds); the
-// hardware's approximations are off by 2^-22 for each u and 2^-23 for the quotient, and each
-// rounding by 2^-24: under |g| 2^-23 + 2^-20, where a code keeps four bits.  (Taking the rounding
-// out of the exponent by an fma: under 2^-19 for every g, 45.6 against 43.3 us for 4096 x 14336.)
-// A g that is not finite gives NaN or an infinity.
-__device__ __forceinline__ float2 silu_times(float2 g, float2 x) {
+// silu(g) * x = g / (1 + exp(-g)) * x of two values, and the least quotient so far.  The hardware's
+// reciprocal gives 0 below the normal range, from g = -87.3 down; where a quotient is 0 the values
+// are taken from far_silu_times.  Relative error of both: an exponent off by 1.25 * 2^-24 of itself
+// (the product and the constant) shows as |g| 2^-23.7, the hardware's approximations are off by 2^-22
+// for each exponential and 2^-23 for the quotient, each rounding by 2^-24: under |g| 2^-23 + 2^-20,
+// where a code keeps four bits.  A g that is not finite gives NaN or an infinity.
+__device__ __forceinline__ float2 silu_times(float2 g, float2 x, float& least) {
+    constexpr float kC = -1.44269504f;      // -1 / ln 2
+    const float2 t = __fmul2_rn(g, make_float2(kC, kC));
+    float2 e, r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(t.x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(t.y));
+    e = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.x) : "f"(e.x));
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r.y) : "f"(e.y));
+    least = fminf(fminf(r.x, r.y), least);
+    return __fmul2_rn(__fmul2_rn(g, r), x);
+}
+
+// The same with u = exp(-|g| / 2): g / (1 + u^2) * x, for g < 0 times u^2, one u to each factor.
+// Nothing overflows, and no factor leaves the normal range before |g| = 174.
+__device__ __forceinline__ float2 far_silu_times(float2 g, float2 x) {
     constexpr float kC = -0.72134752f;      // -1 / (2 ln 2)
     float2 u, r;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(u.x) : "f"(__fmul_rn(fabsf(g.x), kC)));
@@ -562,7 +588,7 @@ __device__ __forceinline__ float2 silu_times(float2 g, float2 x) {
 
 // Rows as they are or gated, a block per eight lanes.  Blocks are numbered through the rows
 // (fewer than 2^31 per launch).  Six CTAs to an SM for gated rows of 16-bit values: they
-// need the loads of so many in flight (4096 x 14336 43.0 us; 45.1 with five, 50.0 with eight, whose
+// need the loads of so many in flight (4096 x 14336 42.7 us; 43.6 with five, 51.6 with eight, whose
 // 32 registers spill); the others as the compiler has them (0).
 template <class T, bool GATED>
 __global__ void __launch_bounds__(256, GATED && Elem<T>::kBytes == 2 ? 6 : 0) gq_fp8_rows_kernel(const GqFp8Rows p, const uint32_t count, const uint32_t mul,
@@ -583,10 +609,21 @@ __global__ void __launch_bounds__(256, GATED && Elem<T>::kBytes == 2 ? 6 : 0) gq
         if constexpr (GATED) g.load(p.gate + (row * p.ld_gate + col) * E, wide);
     }
     float2 y[8];
+    float least = 1.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         y[i] = x.get(i);
-        if constexpr (GATED) y[i] = silu_times(g.get(i), y[i]);
+        if constexpr (GATED) y[i] = silu_times(g.get(i), y[i], least);
+    }
+    if constexpr (GATED) {
+        // loaded again, a pair at a time, so that this way costs no registers
+        if (least == 0.0f) {
+            const uint8_t* const from_x = p.x + (row * p.ld_x + col) * E;
+            const uint8_t* const from_g = p.gate + (row * p.ld_gate + col) * E;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                y[i] = far_silu_times(Raw16<T>::load2(from_g + 2 * i * E), Raw16<T>::load2(from_x + 2 * i * E));
+        }
     }
     uint32_t byte;
     const uint4 c = quantize_block(y, byte);

@@ -60,3 +60,27 @@ def test_gates_that_are_not_finite():
     c = fp8.quantize_fp8(torch.ones(2, 128, device="cuda"), gate=g).codes.float().cpu()
     assert torch.isnan(c[0, :3]).all() and not torch.isnan(c[0, 3:]).any() and not torch.isnan(c[1]).any()
     assert float(c[0, 3]) != 0 and float(c[1, 0]) == 224 and float(c[1, 1]) == 0
+
+
+@pytest.mark.parametrize("dtype", FLOATS)
+@pytest.mark.parametrize("strided", [False, True])
+def test_far_gates_among_ordinary_ones(dtype, strided):
+    """Some lanes of a warp with far gates and some without, on rows that start on 32 bytes and off
+    them, with a ragged last block; and a block of far gates beside ordinary blocks."""
+    gen = torch.Generator("cuda").manual_seed(3)
+    rows, cols = 37, 416
+    pad = 16 // torch.empty(0, dtype=dtype).element_size() if strided else 0
+    wide = torch.zeros(2, rows, cols + 2 * pad, dtype=dtype, device="cuda")
+    x, g = wide[0, :, pad:pad + cols], wide[1, :, pad:pad + cols]
+    x.copy_(torch.randn(rows, cols, device="cuda", generator=gen))
+    gates = torch.randn(rows, cols, device="cuda", generator=gen) * 4
+    far = torch.rand(rows, cols, device="cuda", generator=gen) < 0.02
+    g.copy_(torch.where(far, -87.0 - 10 * torch.rand(rows, cols, device="cuda", generator=gen), gates))
+    g[5, 128:256] = -89
+    g[6, 384:] = -88
+    q = fp8.quantize_fp8(x, gate=g)
+    pd = torch.nn.functional.pad
+    whole = check(pd(x, (0, 512 - cols)), pd(g, (0, 512 - cols)))
+    assert torch.equal(q.codes.view(torch.uint8), whole.codes.view(torch.uint8)[:, :cols])
+    assert torch.equal(q.scales.view(torch.uint8), whole.scales.view(torch.uint8))
+    assert bool((q.codes.float()[5, 128:256] != 0).any()) and bool((q.codes.float()[6, 384:] != 0).any())

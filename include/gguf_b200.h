@@ -254,7 +254,8 @@ GQ_API int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* 
 GQ_API int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream);
 
 /* RMS norm of rows, quantized: h = x + residual rounded to the input type (h = x when
- * residual is NULL), y = h / sqrt(mean(h^2) + eps) * weight in f32, y as e4m3 codes
+ * residual is NULL), y = h / sqrt(mean(h^2) + eps) * weight in f32 (squares included: a row
+ * whose squares overflow gives zeros), y as e4m3 codes
  * (rows, cols) with one scale per 1 x 128 block (rows, ceil(cols/128)).  dtype (of x,
  * residual and sum): GQ_TYPE_F32, F16 or BF16; weight: f32 (cols).  sum receives h when
  * residual is given and may be residual or x itself.  cols a multiple of 32; rows and
@@ -264,8 +265,9 @@ GQ_API int gq_rms_norm_fp8(int32_t dtype, const void* x, int64_t ld_x, const voi
                            const float* weight, float eps, int64_t rows, int64_t cols, void* sum, int64_t ld_sum,
                            uint8_t* codes, int64_t ld_codes, uint8_t* scales, int64_t ld_scales, void* stream);
 
-/* Rows quantized the same way: x, or silu(gate) * x = gate / (1 + exp(-gate)) * x in f32 when
- * gate is given.  Same types and alignment. */
+/* Rows quantized the same way: x, or silu(gate) * x = gate / (1 + exp(-gate)) * x when gate is
+ * given, to |gate| 2^-23 + 2^-20 of the formula's value for |gate| < 174.  Same types and
+ * alignment. */
 GQ_API int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const void* gate, int64_t ld_gate,
                            int64_t rows, int64_t cols, uint8_t* codes, int64_t ld_codes, uint8_t* scales,
                            int64_t ld_scales, void* stream);

@@ -9,7 +9,7 @@
 // weights' traffic: a CTA streams its 128 rows through a ring of 128-column tiles.  Where
 // there are too few row tiles for the SMs, a cluster of 2 to 8 CTAs splits k and adds the
 // partial sums over distributed shared memory in a fixed order.  Measured: 1 x 28672 x 4096 in
-// 20.2 us (5.8 TB/s, 89% of the copy rate), 1 x 4096 x 4096 in 6.0 us, of which the weights'
+// 20.1 us (5.8 TB/s, 89% of the copy rate), 1 x 4096 x 4096 in 5.8 us, of which the weights'
 // bytes are 2.6 and the rest set-up, one round of loads and the join.
 #include <cuda.h>
 #include <cuda_bf16.h>
@@ -322,8 +322,8 @@ __global__ void __launch_bounds__(Narrow<BN, T>::kThreads) gq_matmul_narrow(cons
 // the weights' rows, so a pair reads as much from L2 as one CTA with a tile half as wide.
 // The first 8 warps (16 for f32 outputs) drain the accumulators into registers, release them and
 // then store; of the last three, one loads tiles, one (of the first CTA) issues the matrix
-// instructions and one stages the scales.  Measured: 8192 x 28672 x 4096 in 656 us (2.9 PFLOP/s)
-// in runs of a few ms; held for a second the board's 1000 W bring it to 750-800 us.
+// instructions and one stages the scales.  Measured: 8192 x 28672 x 4096 in 650 us (2.9 PFLOP/s)
+// in runs of a few ms; held for a second the board's 1000 W bring it to 760-780 us.
 
 // A tile's scales as they lie in memory: 128 rows of the tokens' and two of the weights', for all
 // of k.  They come by bulk copies, the next tile's as soon as this one's are read: the tile loads

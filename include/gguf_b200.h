@@ -248,9 +248,9 @@ GQ_API int gq_quantize_rows(const float* x, int64_t rows, int64_t cols, int8_t* 
  *
  * gq_convert_fp8: a GGUF tensor (any type of gq_convert, perm_heads included; cols a
  * multiple of 32, rows and cols at most 2^31 - 1) to tensor->codes, rows * cols e4m3 bytes, and
- * scales, one per 128 x 128 block: (ceil(rows/128), ceil(cols/128)), row-major.  The values quantized are the f32
- * ones of GQ_OUT_F32.  tensor->scales, values and diag are not used.  src and codes 16-byte
- * aligned. */
+ * scales, one per 128 x 128 block: (ceil(rows/128), ceil(cols/128)), row-major.  The values
+ * quantized are the f32 ones of GQ_OUT_F32.  tensor->scales, values and diag are not used.  src
+ * and codes 16-byte aligned. */
 GQ_API int gq_convert_fp8(const gq_tensor_t* tensor, uint8_t* scales, void* stream);
 
 /* RMS norm of rows, quantized: h = x + residual rounded to the input type (h = x when
@@ -274,10 +274,11 @@ GQ_API int gq_quantize_fp8(int32_t dtype, const void* x, int64_t ld_x, const voi
 
 /* out (m, n) = a (m, k) * b (n, k)^T + bias (n, f32, or NULL), accumulated in f32 and rounded
  * once to dtype (GQ_TYPE_F32, F16 or BF16).  The tensor cores truncate as they accumulate; for
- * f32 outputs they take sums of at most 6144 columns, which are added with rounding.  a: e4m3 with one scale per 1 x 128 block,
- * a_scales (m, ceil(k/128)); b: e4m3 with one scale per 128 x 128 block, b_scales
- * (ceil(n/128), ceil(k/128)).  k a multiple of 32; m, n and k at most 2^31 - 513; every row of a
- * and b starts on a 16-byte boundary, out and bias are aligned to their elements. */
+ * f32 outputs they take sums of at most 6144 columns, which are added with rounding.  a: e4m3
+ * with one scale per 1 x 128 block, a_scales (m, ceil(k/128)); b: e4m3 with one scale per
+ * 128 x 128 block, b_scales (ceil(n/128), ceil(k/128)).  k a multiple of 32; m, n and k at most
+ * 2^31 - 513; every row of a and b starts on a 16-byte boundary, out and bias are aligned to
+ * their elements. */
 GQ_API int gq_matmul_fp8(const uint8_t* a, int64_t ld_a, const uint8_t* a_scales, int64_t ld_a_scales,
                          const uint8_t* b, int64_t ld_b, const uint8_t* b_scales, int64_t ld_b_scales,
                          const float* bias, int64_t m, int64_t n, int64_t k, int32_t dtype, void* out,

@@ -50,8 +50,8 @@ __device__ __forceinline__ void bulk(uint32_t dst, const void* src, int bytes, u
 }
 
 // A box in this CTA's shared memory to column x and row y of a 2-D tensor map; what lies outside
-// the tensor is left out, in whole 16 bytes: the tensor's rows have to end on such a boundary.  store_read: until the thread's stores have read their boxes;
-// store_done: until they are complete.
+// the tensor is left out, in whole 16 bytes: the tensor's rows have to end on such a boundary.
+// store_read: until the thread's stores have read their boxes; store_done: until they are complete.
 __device__ __forceinline__ void store_tile(const CUtensorMap* map, int x, int y, uint32_t src) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];\n\tcp.async.bulk.commit_group;" ::"l"(map),
                  "r"(x), "r"(y), "r"(src)
